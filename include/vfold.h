@@ -379,6 +379,68 @@ int vf_quantize_fold(vf_ctx* ctx, const vf_content* base, const vf_quant_spec* s
                      const vf_quant_outputs* outs, vf_stats* stats, char* err, size_t errlen);
 
 /* ------------------------------------------------------------------ */
+/* 8-bit floating-point blocks                                         */
+/* ------------------------------------------------------------------ */
+/* A matrix (or a stack of `count` matrices) of 8-bit floats with one fp32 scale per block of 128 columns: element
+ * (i, r, c) stands for code * scale with
+ *     code  = codes[i * matrix_stride + r * ld + c]
+ *     scale = scales[i * scale_matrix_stride + (r / block_rows) * scale_row_stride + (c / 128) * scale_col_stride]
+ * block_rows is 128 for weights (one scale per 128 x 128 block) and 1 for activations (one per 128 columns of a
+ * row). The last block of a row or column may be short. ld = 0 stands for `cols`, matrix_stride = 0 for rows * ld,
+ * and three scale strides of 0 for a dense array [count][row blocks][column blocks]. Strides count elements, are
+ * not negative and let no two elements meet. The reference's quantized types hold one scale per index of one axis
+ * (!quant.uniform<storage:expressed:axis>); this is the form for which the library's own products exist. */
+#define VF_BLOCK_COLS 128
+typedef struct vf_block_matrix {
+    int32_t dtype;      /* VF_DT_F8E4M3FN or VF_DT_F8E5M2 */
+    int32_t block_rows; /* 1 or 128 */
+    int32_t mem_kind;   /* vf_mem_kind of codes and scales; in host memory both arrays are without gaps */
+    int32_t reserved;
+    int64_t count, rows, cols; /* count, cols >= 1; rows >= 0 */
+    int64_t ld;
+    int64_t matrix_stride;
+    int64_t scale_row_stride, scale_col_stride, scale_matrix_stride;
+    void* codes;
+    uint64_t codes_bytes; /* bytes behind `codes` */
+    float* scales;
+    uint64_t scales_bytes;
+} vf_block_matrix;
+
+/* Quantises `base` (plain f32 / f16 / bf16, [rows, cols] or [count, rows, cols], row r of matrix i starting at
+ * element (i * rows + r) * base_ld; base_ld = 0 stands for cols) into `out`, whose shape must agree:
+ *     scale = max(fl(absmax of the block / L), 2^-126)      L = 448 (e4m3), 57344 (e5m2)
+ *     code  = nearest 8-bit float, ties to even, of fl(x * fl(1 / scale))
+ * so the largest magnitude of a block becomes +-L and a block of zeros gets the scale 2^-126. Bytes of `out` between
+ * rows are left as they are. A NaN gives VF_ERR_NAN, an infinity VF_ERR_QUANT_RANGE, both after the kernel ran (the
+ * block's outputs are then unspecified, the others are complete). */
+int vf_quantize_blocks(vf_ctx* ctx, const vf_content* base, int64_t base_ld, const vf_block_matrix* out, vf_stats* stats,
+                       char* err, size_t errlen);
+
+/* The values of `in` as `dst_dtype` (VF_DT_F32 / F16 / BF16): fl32(code * scale), rounded to nearest even, overflow to
+ * infinity. Row r of matrix i starts at element (i * rows + r) * dst_ld (0 = cols); what lies between rows is left as it is
+ * (in host memory dst_ld must be cols). */
+int vf_dequantize_blocks(vf_ctx* ctx, const vf_block_matrix* in, void* dst, int32_t dst_dtype, int64_t dst_ld,
+                         uint64_t dst_bytes, int dst_mem_kind, vf_stats* stats, char* err, size_t errlen);
+
+/* y[m][n] = sum over k of x[m][k] * w[n][k]: activations x [M, K] with block_rows 1, weights w [N, K] with block_rows
+ * 128 (either 8-bit type on either side), y as `out_dtype` (VF_DT_F32 / F16 / BF16) with rows `out_ld` elements apart
+ * (0 = N). Per 128 columns the codes are multiplied and summed in fp32, the sum is scaled by the product of the two scales
+ * and added in fp32; y is rounded once, to nearest even, overflow to infinity. Everything lives in DEVICE memory;
+ * M = 0 or N = 0 writes nothing. Operands whose codes start on 16-byte boundaries with `ld` (and matrix_stride) a
+ * multiple of 16 run on the tensor cores, others on a plain kernel that is tens of times slower. */
+int vf_matmul_blocks(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matrix* w, void* out, int32_t out_dtype,
+                     int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err, size_t errlen);
+
+/* The product grouped by expert: w holds w->count matrices [N, K], and rows offsets[e] .. offsets[e + 1] of x are
+ * multiplied by matrix e into the same rows of `out`. `offsets` [w->count + 1] lies in DEVICE memory, starts at 0 or
+ * later, does not decrease and ends at or before x->rows; an expert may have no rows. Rows outside
+ * offsets[0] .. offsets[count] are left as they are. Offsets that break these rules give VF_ERR_RANGE after the
+ * kernel ran; they are clamped to them, so nothing outside the operands is touched. */
+int vf_matmul_blocks_grouped(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matrix* w, const int64_t* offsets, void* out,
+                             int32_t out_dtype, int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err,
+                             size_t errlen);
+
+/* ------------------------------------------------------------------ */
 /* sparsity                                                            */
 /* ------------------------------------------------------------------ */
 

@@ -119,6 +119,14 @@ class QuantOutputs(C.Structure):
                 ("dequant_dtype", C.c_int32), ("reserved2", C.c_int32), ("dequant_bytes", C.c_uint64)]
 
 
+class BlockMatrix(C.Structure):
+    _fields_ = [("dtype", C.c_int32), ("block_rows", C.c_int32), ("mem_kind", C.c_int32), ("reserved", C.c_int32),
+                ("count", C.c_int64), ("rows", C.c_int64), ("cols", C.c_int64), ("ld", C.c_int64),
+                ("matrix_stride", C.c_int64), ("scale_row_stride", C.c_int64), ("scale_col_stride", C.c_int64),
+                ("scale_matrix_stride", C.c_int64), ("codes", C.c_void_p), ("codes_bytes", C.c_uint64),
+                ("scales", C.c_void_p), ("scales_bytes", C.c_uint64)]
+
+
 class WeightsTableDesc(C.Structure):
     _fields_ = [("in_elem", ElemType), ("out_elem", ElemType), ("weights_elem", ElemType), ("oc", C.c_int64),
                 ("weights_ptrs", C.POINTER(C.c_int32)), ("sparsity_ptrs", C.POINTER(C.c_int32)),
@@ -306,6 +314,42 @@ def make_transforms(items):
     for i, t in enumerate(items):
         arr[i] = t
     return arr
+
+
+VF_BLOCK_COLS = 128
+
+
+def block_matrix(codes, scales, dtype, block_rows, rows, cols, count=1, ld=0, matrix_stride=0, scale_row_stride=0,
+                 scale_col_stride=0, scale_matrix_stride=0, mem_kind=VF_MEM_DEVICE, codes_bytes=None, scales_bytes=None):
+    """Build a vf_block_matrix. `codes` and `scales` are raw pointers (device), or numpy arrays (host; keep them alive).
+    Byte sizes that are not given are those of the arrays, or, for raw pointers, exactly what the shape and strides span
+    (the caller answers for the buffers being that large). With `count` > 1 and scale strides of which the matrix stride
+    is missing, the matrices' scales follow one another."""
+    m = BlockMatrix()
+    row_blocks, col_blocks = -(-rows // block_rows), -(-cols // VF_BLOCK_COLS)
+    if (scale_row_stride or scale_col_stride) and not scale_matrix_stride:
+        scale_matrix_stride = row_blocks * col_blocks
+    m.dtype, m.block_rows, m.mem_kind, m.count, m.rows, m.cols = dtype, block_rows, mem_kind, count, rows, cols
+    m.ld, m.matrix_stride = ld, matrix_stride
+    m.scale_row_stride, m.scale_col_stride, m.scale_matrix_stride = scale_row_stride, scale_col_stride, scale_matrix_stride
+    for name, x, given in (("codes", codes, codes_bytes), ("scales", scales, scales_bytes)):
+        if isinstance(x, np.ndarray):
+            if not x.flags["C_CONTIGUOUS"]:
+                raise ValueError(f"{name}: the array has to be C-contiguous")
+            setattr(m, name, x.ctypes.data)
+            n = x.nbytes
+        else:
+            setattr(m, name, x)
+            if name == "codes":
+                step = ld or cols
+                n = (count - 1) * (matrix_stride or rows * step) + (rows - 1) * step + cols if rows > 0 else 0
+            else:
+                strides = (scale_matrix_stride, scale_row_stride, scale_col_stride)
+                if not any(strides):
+                    strides = (row_blocks * col_blocks, col_blocks, 1)
+                n = 4 * (1 + sum((e - 1) * st for e, st in zip((count, row_blocks, col_blocks), strides))) if rows > 0 else 0
+        setattr(m, name + "_bytes", n if given is None else given)
+    return m
 
 
 class FolderOptions(C.Structure):

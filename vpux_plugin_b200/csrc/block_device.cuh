@@ -1,0 +1,131 @@
+// Device code shared by the kernels on 8-bit floating-point blocks: conversions, and the walk over the tiles of a
+// product whose rows are grouped by expert.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "blocks.h"
+#include "device_utils.cuh"
+
+namespace vf {
+
+constexpr float kSmallestScale = 1.1754943508222875e-38f;  // 2^-126
+
+__host__ __device__ inline float largest_code(bool e5m2) {
+    return e5m2 ? 57344.f : 448.f;
+}
+
+// Two values to two 8-bit codes (lo in the low byte): nearest, ties to even, magnitudes beyond the largest saturate.
+template <bool E5M2>
+__device__ __forceinline__ uint32_t to_codes(float lo, float hi) {
+    uint16_t r;
+    if constexpr (E5M2) asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// Two 8-bit codes to floats; exact (every value of either type is an fp16 number).
+__device__ __forceinline__ float2 from_codes(uint32_t two, bool e5m2) {
+    if (e5m2) {  // e5m2 is the upper half of an fp16
+        const uint32_t h = __byte_perm(two, 0u, 0x1404);
+        return __half22float2(*reinterpret_cast<const __half2*>(&h));
+    }
+    uint32_t h;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(two)));
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// fp32 results to the output type: nearest, ties to even, overflow to infinity. (The fold's own bf16 conversion drops
+// half of the ties downwards as the reference does; these operators have no such model and round as IEEE 754 says.)
+template <class T>
+__device__ __forceinline__ T to_wide(float v);
+template <>
+__device__ __forceinline__ float to_wide<float>(float v) {
+    return v;
+}
+template <>
+__device__ __forceinline__ __half to_wide<__half>(float v) {
+    return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 to_wide<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// Walks the tiles of a product in ascending order. A tile is `bm` rows of one expert by one of `n_tiles` column tiles;
+// the tiles of expert e come before those of e + 1, and within an expert the row tiles of a column tile follow one
+// another, so that tiles which run at the same time share the weights. Without offsets all rows form one group. Every method is
+// called by whole warps. Offsets are read 32 at a time, one expert per lane; they are clamped into the operand, and
+// offsets that had to be clamped set a flag.
+struct TileWalk {
+    const int64_t* offsets;
+    int* flags;
+    int experts, bm, n_tiles;
+    int64_t rows;
+    int e0;                // expert of lane 0
+    int64_t base;          // tiles before expert e0
+    int64_t through;       // tiles of experts e0 .. e0 + lane
+    int lo, hi;            // this lane's rows
+    // the tile found
+    int expert, row0, row_end, n_tile;
+
+    __device__ __forceinline__ void load() {
+        const int e = e0 + int(threadIdx.x & 31);
+        lo = hi = 0;
+        if (!offsets) {
+            if (e == 0) hi = int(rows);
+        } else if (e < experts) {
+            const int64_t a = offsets[e], b = offsets[e + 1];
+            const int64_t ca = a < 0 ? 0 : (a > rows ? rows : a), cb = b < ca ? ca : (b > rows ? rows : b);
+            if (a != ca || b != cb) set_flag(flags, VF_FLAG_OFFSETS);
+            lo = int(ca);
+            hi = int(cb);
+        }
+        through = int64_t((hi - lo + bm - 1) / bm) * n_tiles;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, through, d);
+            if (int(threadIdx.x & 31) >= d) through += o;
+        }
+    }
+    __device__ __forceinline__ void start(const int64_t* offs, int n_experts, int64_t n_rows, int tile_rows, int col_tiles, int* err_flags) {
+        offsets = offs;
+        experts = n_experts;
+        rows = n_rows;
+        bm = tile_rows;
+        n_tiles = col_tiles;
+        flags = err_flags;
+        e0 = 0;
+        base = 0;
+        load();
+    }
+    // Finds tile `t` (not below the one found before); false behind the last tile.
+    __device__ __forceinline__ bool find(int64_t t) {
+        for (;;) {
+            const int64_t here = __shfl_sync(0xffffffffu, through, 31);
+            if (t - base < here) break;
+            base += here;
+            e0 += 32;
+            if (e0 >= experts) {
+                e0 -= 32;  // a later call ends here again
+                base -= here;
+                return false;
+            }
+            load();
+        }
+        const int64_t rel = t - base;
+        const int src = __ffs(__ballot_sync(0xffffffffu, through > rel)) - 1;
+        const int l = __shfl_sync(0xffffffffu, lo, src), h = __shfl_sync(0xffffffffu, hi, src);
+        const int64_t before = src ? __shfl_sync(0xffffffffu, through, src ? src - 1 : 0) : 0;
+        const int m_tiles = (h - l + bm - 1) / bm;
+        const int in_expert = int(rel - before);
+        n_tile = in_expert / m_tiles;
+        expert = e0 + src;
+        row0 = l + (in_expert - n_tile * m_tiles) * bm;
+        row_end = h;
+        return true;
+    }
+};
+
+}  // namespace vf

@@ -284,7 +284,7 @@ struct vf_ctx {
 
 namespace vf {
 
-constexpr int kNumFlags = 8;
+constexpr int kNumFlags = 10;
 
 // Multiprocessors of the current device (queried once per device): grid-stride launches are capped at a few
 // waves of it.

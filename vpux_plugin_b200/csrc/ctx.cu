@@ -168,6 +168,9 @@ void flags_check(vf_ctx* ctx) {
     if (f[4]) raise(VF_ERR_ALIGNMENT, "weights table: pointer must be a multiple of 16");
     if (f[5]) raise(VF_ERR_NAN, "Quantize met a NaN: its conversion to an integer is undefined in the reference");
     if (f[6]) raise(VF_ERR_NOT_NORMAL, "Taking inverse of a non-normal (e.g. zero/nan/...) float");
+    if (f[7]) raise(VF_ERR_QUANT_RANGE, "an infinite value cannot be quantised");
+    if (f[8]) raise(VF_ERR_RANGE, "row offsets of a grouped product decrease or leave the operand");
+    if (f[9]) raise(VF_ERR_CUDA, "a kernel gave up waiting for its data: the results are not complete");
 }
 
 }  // namespace vf

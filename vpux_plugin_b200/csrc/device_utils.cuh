@@ -22,7 +22,10 @@ enum : int {
     VF_FLAG_TABLE_RANGE = 3,   // weights table: post-shift needed / bias outside int32
     VF_FLAG_TABLE_ALIGN = 4,   // weights table: pointer not 16-byte aligned
     VF_FLAG_NAN = 5,           // NaN met where the reference's behaviour is undefined
-    VF_FLAG_NOT_NORMAL = 6     // ScalarMultInverse of zero, a subnormal, an infinity or NaN
+    VF_FLAG_NOT_NORMAL = 6,    // ScalarMultInverse of zero, a subnormal, an infinity or NaN
+    VF_FLAG_INFINITE = 7,      // an infinity among the values of a block that has to be quantised
+    VF_FLAG_OFFSETS = 8,       // row offsets of a grouped product that decrease or leave the operand
+    VF_FLAG_GAVE_UP = 9        // a wait inside a kernel ran into its time limit
 };
 
 __device__ __forceinline__ void set_flag(int* flags, int slot) {

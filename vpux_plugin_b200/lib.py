@@ -31,6 +31,13 @@ def _load():
                  "vf_nnz_per_oc", "vf_sparsify", "vf_sparsify_batch", "vf_weights_table", "vf_weights_table_batch", "vf_synth_fill", "vf_plan_shards",
                  "vf_ctx_create", "vf_ctx_synchronize", "vf_abi_version", "vf_ctx_device", "vf_fold_batch", "vf_max_intermediate_size"):
         getattr(lib, name).restype = C.c_int
+    # calls of a few microseconds: their arguments are converted by declared types
+    p, i32, i64, u64, tail = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, [C.c_void_p, C.c_char_p, C.c_size_t]
+    for name, args in (("vf_quantize_blocks", [p, p, i64, p]), ("vf_dequantize_blocks", [p, p, p, i32, i64, u64, i32]),
+                       ("vf_matmul_blocks", [p, p, p, p, i32, i64, u64]),
+                       ("vf_matmul_blocks_grouped", [p, p, p, p, p, i32, i64, u64])):
+        getattr(lib, name).restype = C.c_int
+        getattr(lib, name).argtypes = args + tail
     lib.vf_ctx_destroy.restype = None
     lib.vf_ctx_destroy.argtypes = [C.c_void_p]
     lib.vf_ctx_stream.restype = C.c_void_p
@@ -283,6 +290,35 @@ class Library:
         """jobs: ctypes array of abi.WeightsTableJob (tables in memory of kind `out_mem_kind`)."""
         err = self._err()
         st = self.lib.vf_weights_table_batch(self.ctx, jobs, len(jobs), int(out_mem_kind), err, C.c_size_t(512))
+        self._check(st, err)
+
+    # -- 8-bit floating-point blocks ----------------------------------------------------------------------
+    def quantize_blocks(self, content, out, base_ld=0):
+        """vf_quantize_blocks: `content` (abi.Content) into `out` (abi.BlockMatrix)."""
+        err = self._err()
+        st = self.lib.vf_quantize_blocks(self.ctx, C.byref(content), base_ld, C.byref(out), C.byref(self.last_stats), err, 512)
+        self._check(st, err)
+
+    def dequantize_blocks(self, matrix, dst, dst_dtype, dst_bytes, dst_ld=0, dst_mem_kind=abi.VF_MEM_DEVICE):
+        """vf_dequantize_blocks: the values of `matrix` as `dst_dtype` at `dst` (raw pointer, or numpy array in host memory)."""
+        err = self._err()
+        st = self.lib.vf_dequantize_blocks(self.ctx, C.byref(matrix), _ptr(dst), dst_dtype, dst_ld, dst_bytes, dst_mem_kind,
+                                           C.byref(self.last_stats), err, 512)
+        self._check(st, err)
+
+    def matmul_blocks(self, x, w, out, out_dtype, out_bytes, out_ld=0):
+        """vf_matmul_blocks: out[m][n] = sum_k x[m][k] * w[n][k]; `out` is a raw device pointer."""
+        err = self._err()
+        st = self.lib.vf_matmul_blocks(self.ctx, C.byref(x), C.byref(w), out, out_dtype, out_ld, out_bytes, C.byref(self.last_stats),
+                                       err, 512)
+        self._check(st, err)
+
+    def matmul_blocks_grouped(self, x, w, offsets, out, out_dtype, out_bytes, out_ld=0):
+        """vf_matmul_blocks_grouped: rows offsets[e] .. offsets[e + 1] of x times matrix e of w; `offsets` (w.count + 1
+        int64) and `out` are raw device pointers."""
+        err = self._err()
+        st = self.lib.vf_matmul_blocks_grouped(self.ctx, C.byref(x), C.byref(w), offsets, out, out_dtype, out_ld, out_bytes,
+                                               C.byref(self.last_stats), err, 512)
         self._check(st, err)
 
     def synth_fill_device(self, spec, dst_ptr, count):
