@@ -2,6 +2,7 @@
 //
 //   y[m][n] = sum over column blocks b of  (sx[m][b] * sw[n / 128][b]) * sum over k in b of cx[m][k] * cw[n][k]
 #include "block_device.cuh"
+#include "tensor_core.cuh"
 
 namespace vf {
 
@@ -75,12 +76,341 @@ void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
     k_matmul_blocks_plain<T><<<unsigned(std::min<int64_t>(tiles, 8 * ctx->sm_count)), 256, 0, ctx->stream>>>(p, int(n_tiles), ctx->d_flags);
 }
 
+
+// ---- tensor cores ------------------------------------------------------------------------------------------------------
+// The weights are the 128-row operand: a tile holds 128 outputs n (one row block of the weights, hence ONE weight scale
+// per column block) of BN activations m. The products of one column block (four steps of 32 k) start from zero in one of NBUF
+// accumulators in tensor memory; while the tensor core fills the next one, the epilogue warps read it, multiply it by the
+// column block's scales and add it to the running sums, which stay in registers:  sum[m] += part[m] * (sx[m] * sw).
+// With BN = 256 that is 128 sums per thread in 8 warps.
+//
+// Warps: 0 copies tiles in (bulk tensor copies into a ring of STAGES), 1 issues the matrix instructions, 2 and 3 put the
+// scales sx * sw of a column block next to its accumulator, 4 and up are the epilogue, whose warps read the 32 lanes
+// of tensor memory that belong to their position in their group of four.
+//
+// Few rows make few tiles: the column blocks of a tile are then spread over the CTAs of a cluster, which add up their
+// sums through each other's shared memory, every CTA for its share of the tile's rows of activations, always in the order of
+// the ranks.
+template <int BN_, int STAGES_, int NBUF_, int GROUPS_, int PER_SM_>
+struct Shape {
+    static constexpr int BN = BN_, STAGES = STAGES_, NBUF = NBUF_, GROUPS = GROUPS_, PER_SM = PER_SM_;
+    static constexpr int kThreads = 128 + 128 * GROUPS;
+    static constexpr int kCols = BN / GROUPS;               // columns (activations) per epilogue warp
+    static constexpr int kScaleWarps = BN >= 64 ? 2 : 1;
+    static constexpr int kScalesPerLane = (BN / kScaleWarps + 31) / 32;
+    static constexpr int kStageBytes = (128 + BN) * kBlock;
+    static constexpr int kTmem = NBUF * BN < 32 ? 32 : NBUF * BN;
+    static constexpr bool kSplits = BN <= 32;               // clusters share a tile's column blocks
+    static constexpr int kRing = STAGES * kStageBytes;
+    static constexpr int kScales = NBUF * BN * 4;
+    static constexpr int kReduce = kSplits ? 128 * BN * 4 : 0;
+    static constexpr int kBars = 2 * STAGES + 3 * NBUF + 3;
+    static constexpr int kSmem = 1024 + kRing + kScales + kReduce + kBars * 8 + 16;
+};
+
+template <class S, class T>
+__global__ void __launch_bounds__(S::kThreads, S::PER_SM)
+    k_matmul_blocks(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ BlockProduct p, int n_tiles,
+                    uint32_t idesc, int* flags) {
+    constexpr int BN = S::BN, STAGES = S::STAGES, NBUF = S::NBUF;
+    extern __shared__ char raw[];
+    char* const base = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;  // the swizzle works on 1024-byte units
+    char* const ring = base;
+    float* const scales = reinterpret_cast<float*>(base + S::kRing);
+    float* const partial = reinterpret_cast<float*>(base + S::kRing + S::kScales);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(base + S::kRing + S::kScales + S::kReduce);
+    uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bars + S::kBars);
+    volatile int* const gave_up = reinterpret_cast<volatile int*>(tmem_at + 1);
+    const uint32_t full = smem_addr(bars), empty = full + 8 * STAGES;                      // ring
+    const uint32_t done = empty + 8 * STAGES, scaled = done + 8 * NBUF, taken = scaled + 8 * NBUF;  // accumulators
+    const uint32_t parts_full = taken + 8 * NBUF, parts_free = parts_full + 8, drained = parts_free + 8;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ranks = S::kSplits ? cluster_size() : 1, rank = S::kSplits ? cluster_rank() : 0;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            bar_init(full + 8 * i, 1);
+            bar_init(empty + 8 * i, 1);
+        }
+        for (int i = 0; i < NBUF; ++i) {
+            bar_init(done + 8 * i, 1);
+            bar_init(scaled + 8 * i, S::kScaleWarps);
+            bar_init(taken + 8 * i, 4 * S::GROUPS);
+        }
+        bar_init(parts_full, 4 * ranks);
+        bar_init(parts_free, 4 * ranks);
+        bar_init(drained, 1);
+        *gave_up = 0;
+        bar_init_fence();
+        tma_prefetch_map(&xmap);
+        tma_prefetch_map(&wmap);
+    }
+    if (warp == 2) tmem_alloc(smem_addr(tmem_at), S::kTmem);
+    tc_fence_before();
+    __syncthreads();
+    if (ranks > 1) cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_at;
+
+    const int kbs = int(p.x.col_blocks), kb0 = int(rank * uint32_t(kbs) / ranks), kb1 = int((rank + 1) * uint32_t(kbs) / ranks);
+    const int64_t first = blockIdx.x / ranks, step = gridDim.x / ranks;
+    TileWalk walk;
+    walk.start(p.offsets, p.offsets ? int(p.w.count) : 1, p.x.rows, BN, n_tiles, flags);
+
+    if (warp == 0) {  // ---- copies
+        uint32_t it = 0;
+        bool ok = true;
+        for (int64_t t = first; ok && walk.find(t); t += step) {
+            if (lane == 0) {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const uint32_t s = it % STAGES, bar = full + 8 * s, at = smem_addr(ring) + s * S::kStageBytes;
+                    ok = bar_wait(empty + 8 * s, ((it / STAGES) & 1) ^ 1, gave_up);
+                    if (!ok) break;
+                    bar_expect(bar, S::kStageBytes);
+                    tma_load_3d(at, &wmap, bar, kb * kBlock, walk.n_tile * 128, walk.expert);
+                    tma_load_2d(at + 128 * kBlock, &xmap, bar, kb * kBlock, walk.row0);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, int(ok), 0);
+        }
+        if (ok && lane == 0)  // every arrival at the ring's barriers has happened before the CTA ends
+            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) bar_wait(empty + 8 * (i % STAGES), (i / STAGES) & 1, gave_up);
+        if (!ok && lane == 0)  // the copies in flight land before the CTA ends
+            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
+                const uint64_t t0 = global_ns();
+                while (!bar_try<false>(full + 8 * (i % STAGES), (i / STAGES) & 1) && global_ns() - t0 < kWaitLimitNs) {
+                }
+            }
+    } else if (warp == 1) {  // ---- matrix instructions
+        uint32_t it = 0;
+        bool ok = true;
+        for (int64_t t = first; ok && walk.find(t); t += step) {
+            if (lane == 0) {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const uint32_t s = it % STAGES, b = it % NBUF;
+                    ok = bar_wait(taken + 8 * b, ((it / NBUF) & 1) ^ 1, gave_up) && bar_wait(full + 8 * s, (it / STAGES) & 1, gave_up);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t at = smem_addr(ring) + s * S::kStageBytes;
+                    const uint64_t wd = tc_operand(at), xd = tc_operand(at + 128 * kBlock);
+#pragma unroll
+                    for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8(tmem + b * BN, wd + 2 * k, xd + 2 * k, idesc, k > 0);
+                    tc_commit(empty + 8 * s);
+                    tc_commit(done + 8 * b);
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, int(ok), 0);
+        }
+        if (!ok && lane == 0) {  // the instructions in flight end before their memory is given back
+            tc_commit(drained);
+            const uint64_t t0 = global_ns();
+            while (!bar_try<false>(drained, 0) && global_ns() - t0 < kWaitLimitNs) {
+            }
+        }
+    } else if (warp < 2 + S::kScaleWarps) {  // ---- scales, read four column blocks ahead
+        constexpr int kAhead = 4, kPer = S::kScalesPerLane;
+        const int col0 = (warp - 2) * (BN / S::kScaleWarps) + lane;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int64_t t = first; ok && walk.find(t); t += step) {
+            const float* const sw = p.w.scales + walk.expert * p.w.sms + walk.n_tile * p.w.srs;
+            const float* const sx = p.x.scales + (walk.row0 + col0) * p.x.srs;
+            const int here = walk.row_end - walk.row0 - col0;  // column 32 * i of this lane exists if 32 * i < here
+            float x[kAhead][kPer], w[kAhead];
+            auto load = [&](int kb) {
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    const bool in = kb + a < kb1;
+                    w[a] = in ? sw[(kb + a) * p.w.scs] : 0.f;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) x[a][i] = in && 32 * i < here && col0 + 32 * i < BN ? sx[32 * i * p.x.srs + (kb + a) * p.x.scs] : 0.f;
+                }
+            };
+            load(kb0);
+            for (int kb = kb0; ok && kb < kb1; kb += kAhead) {
+                float v[kAhead][kPer];
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) v[a][i] = __fmul_rn(x[a][i], w[a]);
+                if (kb + kAhead < kb1) load(kb + kAhead);
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a) {
+                    if (kb + a >= kb1 || !ok) break;
+                    const uint32_t b = it % NBUF;
+                    ok = bar_wait(taken + 8 * b, ((it / NBUF) & 1) ^ 1, gave_up);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i)
+                        if (col0 + 32 * i < BN) scales[b * BN + col0 + 32 * i] = v[a][i];
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(scaled + 8 * b);
+                    ++it;
+                }
+            }
+        }
+    } else if (warp >= 4) {  // ---- epilogue
+        constexpr int kCols = S::kCols;
+        const int quarter = warp & 3, col0 = (warp - 4) / 4 * kCols;
+        const uint32_t my_tmem = tmem + (uint32_t(quarter) << 21) + col0;
+        uint32_t it = 0, round = 0;
+        bool ok = true;
+        for (int64_t t = first; ok && walk.find(t); t += step) {
+            uint64_t acc[kCols / 2];
+#pragma unroll
+            for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t b = it % NBUF, ph = (it / NBUF) & 1;
+                ok = bar_wait(scaled + 8 * b, ph, gave_up) && bar_wait(done + 8 * b, ph, gave_up);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                tc_fence_after();
+                const float* const sc = scales + b * BN + col0;
+#pragma unroll
+                for (int c = 0; c < kCols; c += 16) {
+                    uint32_t v[16];
+                    tmem_load_16(v, my_tmem + b * BN + c);
+                    tmem_load_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; i += 4) {
+                        const uint4 s4 = *reinterpret_cast<const uint4*>(sc + c + i);
+                        fma2(acc[(c + i) / 2], pack2(v[i], v[i + 1]), pack2(s4.x, s4.y));
+                        fma2(acc[(c + i) / 2 + 1], pack2(v[i + 2], v[i + 3]), pack2(s4.z, s4.w));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(taken + 8 * b);
+            }
+            if (!ok) break;
+            const int here = walk.row_end - walk.row0;
+            const int n = walk.n_tile * 128 + quarter * 32 + lane;
+            T* const out = static_cast<T*>(p.out) + int64_t(walk.row0) * p.out_ld + n;
+            if (S::kSplits && ranks > 1) {
+                if constexpr (S::kSplits) {
+                    float* const mine = partial + quarter * 32 + lane;
+                    ok = __all_sync(0xffffffffu, bar_wait<true>(parts_free, (round & 1) ^ 1, gave_up));
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < kCols; ++i)
+                        if (i < here) mine[i * 128] = __uint_as_float(uint32_t(acc[i / 2] >> (32 * (i & 1))));
+                    __syncwarp();
+                    if (lane < ranks) bar_arrive_at(parts_full, lane);
+                    ok = __all_sync(0xffffffffu, bar_wait<true>(parts_full, round & 1, gave_up));
+                    if (!ok) break;
+                    for (int i = int(rank); i < here && i < BN; i += int(ranks)) {
+                        float v = 0.f;
+                        for (uint32_t r = 0; r < ranks; ++r) v = __fadd_rn(v, load_from_rank(smem_addr(mine + i * 128), r));
+                        if (n < p.w.rows) out[i * p.out_ld] = to_wide<T>(v);
+                    }
+                    __syncwarp();
+                    if (lane < ranks) bar_arrive_at(parts_free, lane);
+                    ++round;
+                }
+            } else if (n < p.w.rows) {
+#pragma unroll
+                for (int i = 0; i < kCols; ++i)
+                    if (col0 + i < here) out[int64_t(col0 + i) * p.out_ld] = to_wide<T>(__uint_as_float(uint32_t(acc[i / 2] >> (32 * (i & 1)))));
+            }
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 2) tmem_free(tmem, S::kTmem);
+    if (threadIdx.x == 0 && *gave_up) set_flag(flags, VF_FLAG_GAVE_UP);
+    __syncwarp();
+    if (ranks > 1) cluster_sync();  // no CTA ends while another one reads its sums
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled f = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+            raise(VF_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+        return reinterpret_cast<EncodeTiled>(p);
+    }();
+    return f;
+}
+
+// Boxes of `box_rows` rows by 128 columns of a matrix (rank 2) or a stack of them (rank 3); what lies outside reads as zero.
+CUtensorMap map_codes(const Blocks& b, int rank, int box_rows) {
+    CUtensorMap m;
+    const cuuint64_t dim[3] = {cuuint64_t(b.cols), cuuint64_t(b.rows), cuuint64_t(b.count)};
+    const cuuint64_t stride[2] = {cuuint64_t(b.ld), cuuint64_t(b.count > 1 ? b.matrix_stride : b.ld)};
+    const cuuint32_t box[3] = {kBlock, cuuint32_t(box_rows), 1}, one[3] = {1, 1, 1};
+    const CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank), b.codes, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) raise(VF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+    return m;
+}
+
+bool fits_bulk_copies(const Blocks& b) {  // start and pitches of 16-byte units, pitches below 2^40 bytes
+    return (reinterpret_cast<uintptr_t>(b.codes) & 15u) == 0 && b.ld % 16 == 0 && b.ld < (int64_t(1) << 40) &&
+           (b.count == 1 || (b.matrix_stride % 16 == 0 && b.matrix_stride < (int64_t(1) << 40)));
+}
+
+template <class S, class T>
+void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks) {
+    auto kernel = k_matmul_blocks<S, T>;
+    VF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    const int64_t n_tiles = (p.w.rows + 127) / 128;
+    const int64_t tiles = most_row_tiles(p, S::BN) * n_tiles;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(unsigned(std::min<int64_t>(tiles, std::max(1, ctx->sm_count * S::PER_SM / ranks)) * ranks));
+    cfg.blockDim = dim3(S::kThreads);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = ctx->stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = unsigned(ranks);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const uint32_t idesc = tc_f8_shape(p.w.dtype == VF_DT_F8E5M2, p.x.dtype == VF_DT_F8E5M2, S::BN);
+    VF_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_codes(p.x, 2, S::BN), map_codes(p.w, 3, 128), p, int(n_tiles), idesc, ctx->d_flags));
+}
+
+//                     BN, stages, accumulators, epilogue groups of four warps, CTAs per SM
+using Shape16 = Shape<16, 5, 4, 1, 2>;
+using Shape32 = Shape<32, 4, 4, 1, 2>;
+using Shape64 = Shape<64, 4, 4, 1, 2>;
+using Shape128 = Shape<128, 6, 2, 2, 1>;
+using Shape256 = Shape<256, 4, 2, 4, 1>;
+
+template <class T>
+void launch_for(vf_ctx* ctx, const BlockProduct& p) {
+    if (!fits_bulk_copies(p.x) || !fits_bulk_copies(p.w)) return launch_plain<T>(ctx, p);
+    const int64_t rows = p.offsets ? (p.x.rows + p.w.count - 1) / p.w.count : p.x.rows;
+    const int64_t n_tiles = (p.w.rows + 127) / 128;
+    if (rows <= 32) {
+        const int bn = rows <= 16 ? 16 : 32;
+        const int64_t tiles = most_row_tiles(p, bn) * n_tiles;
+        int ranks = 1;
+        while (ranks < 8 && tiles * ranks * 2 <= 2 * ctx->sm_count && p.x.col_blocks >= 4 * ranks) ranks *= 2;
+        if (bn == 16) launch_tensor<Shape16, T>(ctx, p, ranks);
+        else launch_tensor<Shape32, T>(ctx, p, ranks);
+    } else if (rows <= 64) {
+        launch_tensor<Shape64, T>(ctx, p, 1);
+    } else if (rows <= 128) {
+        launch_tensor<Shape128, T>(ctx, p, 1);
+    } else {
+        launch_tensor<Shape256, T>(ctx, p, 1);
+    }
+}
+
 }  // namespace
 
 void launch_matmul_blocks(vf_ctx* ctx, const BlockProduct& p) {
-    if (p.out_dt == VF_DT_F32) launch_plain<float>(ctx, p);
-    else if (p.out_dt == VF_DT_F16) launch_plain<__half>(ctx, p);
-    else launch_plain<__nv_bfloat16>(ctx, p);
+    if (p.out_dt == VF_DT_F32) launch_for<float>(ctx, p);
+    else if (p.out_dt == VF_DT_F16) launch_for<__half>(ctx, p);
+    else launch_for<__nv_bfloat16>(ctx, p);
     VF_CUDA(cudaGetLastError());
     ctx->launches += 1;
 }
