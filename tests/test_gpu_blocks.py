@@ -303,6 +303,27 @@ def test_product(gpu, torch, xt, wt, out_dt):
         check_product(got, *ops, xt, wt, out_dt)
 
 
+@pytest.mark.parametrize("m,n,k,out_ld", [(2300, 2500, 400, 0), (1100, 4099, 272, 0), (4097, 1300, 128, 1301), (1024, 5000, 1600, 5008)])
+def test_product_with_many_tiles(gpu, torch, m, n, k, out_ld):
+    """Enough tiles for every multiprocessor, several each: 256 rows by 256 columns on pairs of them."""
+    rng = np.random.default_rng(24)
+    for xt, wt, out_dt in ((E4M3, E4M3, BF16), (E5M2, E4M3, F32)):
+        ops = operands(rng, m, n, k, xt, wt)
+        got = run_product(gpu, torch, *ops, xt, wt, out_dt, out_ld=out_ld)
+        check_product(got, *ops, xt, wt, out_dt)
+
+
+@pytest.mark.parametrize("offsets,n", [([0, 700, 700, 701, 2000, 2256], 1500), ([7] + [7 + 60 * i for i in range(40)], 1100)])
+def test_grouped_product_with_many_tiles(gpu, torch, offsets, n):
+    rng = np.random.default_rng(25)
+    m, experts = offsets[-1] + 11, len(offsets) - 1
+    ops = operands(rng, m, n, 300, E4M3, E4M3, experts)
+    got = run_product(gpu, torch, *ops, E4M3, E4M3, BF16, offsets=offsets)
+    for e in range(experts):
+        check_product(got, *ops, E4M3, E4M3, BF16, offsets[e], offsets[e + 1], e)
+    assert (got[:offsets[0]] == 3).all() and (got[offsets[-1]:] == 3).all()
+
+
 @pytest.mark.parametrize("m", [3, 70, 300])
 @pytest.mark.parametrize("x_kw,w_kw,out_ld,out_offset", [
     ({"ld": 320, "col_major": False}, {"ld": 336, "col_major": True}, 0, 0),      # scales in the other orders, rows further apart

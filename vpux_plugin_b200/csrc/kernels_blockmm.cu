@@ -84,29 +84,80 @@ void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
 // column block's scales and add it to the running sums, which stay in registers:  sum[m] += part[m] * (sx[m] * sw).
 // With BN = 256 that is 128 sums per thread in 8 warps.
 //
-// Warps: 0 copies tiles in (bulk tensor copies into a ring of STAGES), 1 issues the matrix instructions, 2 and 3 put the
-// scales sx * sw of a column block next to its accumulator, 4 and up are the epilogue, whose warps read the 32 lanes
-// of tensor memory that belong to their position in their group of four.
+// Warps: the first ones are the epilogue, in groups of four that read a quarter of tensor memory's lanes each; then one that
+// copies tiles in (bulk tensor copies into a ring of STAGES) and one that issues the matrix instructions.
 //
 // Few rows make few tiles: the column blocks of a tile are then spread over the CTAs of a cluster, which add up their
 // sums through each other's shared memory, every CTA for its share of the tile's rows of activations, always in the order of
 // the ranks.
-template <int BN_, int STAGES_, int NBUF_, int GROUPS_, int PER_SM_>
-struct Shape {
-    static constexpr int BN = BN_, STAGES = STAGES_, NBUF = NBUF_, GROUPS = GROUPS_, PER_SM = PER_SM_;
-    static constexpr int kThreads = 128 + 128 * GROUPS;
-    static constexpr int kCols = BN / GROUPS;               // columns (activations) per epilogue warp
-    static constexpr int kScaleWarps = BN >= 64 ? 2 : 1;
-    static constexpr int kScalesPerLane = (BN / kScaleWarps + 31) / 32;
-    static constexpr int kStageBytes = (128 + BN) * kBlock;
-    static constexpr int kTmem = NBUF * BN < 32 ? 32 : NBUF * BN;
-    static constexpr bool kSplits = BN <= 32;               // clusters share a tile's column blocks
-    static constexpr int kRing = STAGES * kStageBytes;
-    static constexpr int kScales = NBUF * BN * 4;
-    static constexpr int kReduce = kSplits ? 128 * BN * 4 : 0;
-    static constexpr int kBars = 2 * STAGES + 3 * NBUF + 3;
-    static constexpr int kSmem = 1024 + kRing + kScales + kReduce + kBars * 8 + 16;
+constexpr int kGiven = 72, kTaken = 216;  // registers per thread after the trade: 128 * 72 + 256 * 216 = 384 * 168
+
+enum class Form {
+    kSwap,    // the weights are the 128-row operand, BN activations the other one
+    kSingle,  // 128 activations are the 128-row operand, BN outputs the other one
+    kPair     // the same with 256 activations on a pair of CTAs, which share the BN outputs' weights
 };
+
+template <Form FORM_, int BN_, int STAGES_, int NBUF_, int GROUPS_, int PER_SM_, int LOAD_ = 32>
+struct Shape {
+    static constexpr bool SWAP = FORM_ == Form::kSwap, PAIR = FORM_ == Form::kPair;
+    static constexpr int BN = BN_, STAGES = STAGES_, NBUF = NBUF_, GROUPS = GROUPS_, PER_SM = PER_SM_, LOAD = LOAD_;
+    static constexpr int kCols = BN / GROUPS;               // columns of the accumulator per epilogue warp
+    static constexpr int kTokens = SWAP ? BN : (PAIR ? 256 : 128), kOutputs = SWAP ? 128 : BN;  // a tile's results
+    static constexpr int kScaleWarps = SWAP && BN >= 64 ? 2 : 1;
+    static constexpr int kEpilogue = 4 * GROUPS, kCopies = kEpilogue, kIssue = kEpilogue + 1, kScaling = kEpilogue + 2;  // warps
+    static constexpr bool kTrades = kCols > 64;             // the warps behind the epilogue's give it registers, as a group of four
+    static constexpr int kThreads = 32 * (kEpilogue + (kTrades ? 4 : 2 + kScaleWarps));
+    // activations as the 128-row operand: scales of kAhead column blocks at a time, [kAhead][128] of rows, [2][kAhead] of weights
+    static constexpr int kAhead = 8, kSlots = 2, kSlotBytes = kAhead * 128 * 4 + 2 * kAhead * 4;
+    static constexpr int kScalesPerWarp = BN / kScaleWarps;
+    static constexpr int kScalesPerLane = (kScalesPerWarp + 31) / 32;
+    static constexpr int kRowsB = PAIR ? BN / 2 : BN;       // rows of the second operand that this CTA holds
+    static constexpr int kStageBytes = (128 + kRowsB) * kBlock;
+    static constexpr int kTmem = NBUF * BN < 32 ? 32 : NBUF * BN;
+    static constexpr bool kSplits = SWAP && BN <= 32;       // clusters share a tile's column blocks
+    static constexpr int kRing = STAGES * kStageBytes;
+    static constexpr int kScales = SWAP ? NBUF * BN * 4 : kSlots * kSlotBytes;
+    static constexpr int kExtra = kSplits ? 128 * BN * 4 : (SWAP ? 0 : 4 * GROUPS * 4096);  // partial sums; results on their way out
+    static constexpr int kBars = 2 * STAGES + 3 * NBUF + 3 + 2 * 2 + 2 * kSlots;
+    static constexpr int kSmem = 1024 + kRing + kScales + kExtra + 2 * 16 + kBars * 8 + 16;
+};
+
+// A warp's 32 rows x N results (one row per lane) to memory, 128 bytes of every row at a time: through shared memory, so that
+// eight lanes write one row's 128 bytes, in 16-byte units where every row allows them. `rows` and `cols` of them exist.
+template <class T, int N>
+__device__ __forceinline__ void store_rows(char* stage, T* out, int64_t ld, const uint64_t (&acc)[N / 2], int rows, int cols, int lane) {
+    constexpr int kPer = 16 / sizeof(T), kChunk = 8 * kPer;  // elements per 16 bytes, per 128 bytes
+    const bool aligned = (reinterpret_cast<uintptr_t>(out) & 15u) == 0 && (ld * sizeof(T)) % 16 == 0;
+#pragma unroll
+    for (int c = 0; c < N; c += kChunk) {
+        __syncwarp();  // the chunk before has been read
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            alignas(16) T v[kPer];
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int k = c + u * kPer + i;
+                v[i] = to_wide<T>(__uint_as_float(uint32_t(acc[k / 2] >> (32 * (k & 1)))));
+            }
+            *reinterpret_cast<uint4*>(stage + lane * 128 + ((u ^ lane) & 7) * 16) = *reinterpret_cast<const uint4*>(v);
+        }
+        __syncwarp();
+        if (aligned && c + kChunk <= cols) {
+            const int u = lane & 7;
+#pragma unroll
+            for (int r = lane >> 3; r < 32; r += 4) {
+                const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((u ^ r) & 7) * 16);
+                if (r < rows) *reinterpret_cast<uint4*>(out + r * ld + c + u * kPer) = v;
+            }
+        } else {
+            for (int r = 0; r < rows; ++r)
+#pragma unroll
+                for (int k = lane; k < kChunk; k += 32)
+                    if (c + k < cols) out[r * ld + c + k] = *reinterpret_cast<const T*>(stage + r * 128 + ((k / kPer ^ r) & 7) * 16 + k % kPer * sizeof(T));
+        }
+    }
+}
 
 template <class S, class T>
 __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
@@ -117,16 +168,21 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     char* const base = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;  // the swizzle works on 1024-byte units
     char* const ring = base;
     float* const scales = reinterpret_cast<float*>(base + S::kRing);
-    float* const partial = reinterpret_cast<float*>(base + S::kRing + S::kScales);
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(base + S::kRing + S::kScales + S::kReduce);
+    char* const extra = base + S::kRing + S::kScales;
+    int4* const tiles = reinterpret_cast<int4*>(extra + S::kExtra);  // expert (-1: no more tiles), row0, row_end, n_tile
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(tiles + 2);
     uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bars + S::kBars);
     volatile int* const gave_up = reinterpret_cast<volatile int*>(tmem_at + 1);
     const uint32_t full = smem_addr(bars), empty = full + 8 * STAGES;                      // ring
     const uint32_t done = empty + 8 * STAGES, scaled = done + 8 * NBUF, taken = scaled + 8 * NBUF;  // accumulators
     const uint32_t parts_full = taken + 8 * NBUF, parts_free = parts_full + 8, drained = parts_free + 8;
+    const uint32_t tile_there = drained + 8, tile_read = tile_there + 16;
+    const uint32_t slot_full = tile_read + 16, slot_read = slot_full + 8 * S::kSlots;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t ranks = S::kSplits ? cluster_size() : 1, rank = S::kSplits ? cluster_rank() : 0;
+    const uint32_t ranks = S::kSplits ? cluster_size() : 1, rank = S::kSplits ? cluster_rank() : 0;  // CTAs that share a tile's column blocks
+    const uint32_t half = S::PAIR ? cluster_rank() : 0;
+    const bool in_cluster = S::PAIR || ranks > 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             bar_init(full + 8 * i, 1);
@@ -135,87 +191,120 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         for (int i = 0; i < NBUF; ++i) {
             bar_init(done + 8 * i, 1);
             bar_init(scaled + 8 * i, S::kScaleWarps);
-            bar_init(taken + 8 * i, 4 * S::GROUPS);
+            bar_init(taken + 8 * i, (S::PAIR ? 8 : 4) * S::GROUPS);
         }
         bar_init(parts_full, 4 * ranks);
         bar_init(parts_free, 4 * ranks);
         bar_init(drained, 1);
+        for (int i = 0; i < 2; ++i) {
+            bar_init(tile_there + 8 * i, 1);
+            bar_init(tile_read + 8 * i, S::kEpilogue + 1 + S::kScaleWarps);
+        }
+        for (int i = 0; i < S::kSlots; ++i) {
+            bar_init(slot_full + 8 * i, 32);
+            bar_init(slot_read + 8 * i, S::kEpilogue);
+        }
         *gave_up = 0;
         bar_init_fence();
         tma_prefetch_map(&xmap);
         tma_prefetch_map(&wmap);
     }
-    if (warp == 2) tmem_alloc(smem_addr(tmem_at), S::kTmem);
+    if (warp == S::kIssue) tmem_alloc<S::PAIR>(smem_addr(tmem_at), S::kTmem);
     tc_fence_before();
     __syncthreads();
-    if (ranks > 1) cluster_sync();
+    if (in_cluster) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
 
     const int kbs = int(p.x.col_blocks), kb0 = int(rank * uint32_t(kbs) / ranks), kb1 = int((rank + 1) * uint32_t(kbs) / ranks);
-    const int64_t first = blockIdx.x / ranks, step = gridDim.x / ranks;
-    TileWalk walk;
-    walk.start(p.offsets, p.offsets ? int(p.w.count) : 1, p.x.rows, BN, n_tiles, flags);
+    // The next tile, as the copying warp has found it; by whole warps
+    int4 tile;
+    uint32_t turn = 0;
+    auto next_tile = [&]() {
+        const uint32_t i = turn & 1;
+        if (!__all_sync(0xffffffffu, bar_wait(tile_there + 8 * i, (turn >> 1) & 1, gave_up))) return false;
+        tile = tiles[i];
+        __syncwarp();
+        if (lane == 0) bar_arrive(tile_read + 8 * i);
+        ++turn;
+        return tile.x >= 0;
+    };
 
-    if (warp == 0) {  // ---- copies
+    if (warp >= S::kEpilogue) {
+    if constexpr (S::kTrades) regs_give<kGiven>();
+    if (warp == S::kCopies) {  // ---- finding tiles, copying them in
+        const uint32_t sharing = S::PAIR ? 2 : ranks;
+        TileWalk walk;
+        walk.start(p.offsets, p.offsets ? int(p.w.count) : 1, p.x.rows, S::kTokens, n_tiles, flags);
         uint32_t it = 0;
         bool ok = true;
-        for (int64_t t = first; ok && walk.find(t); t += step) {
+        for (int64_t t = blockIdx.x / sharing; ok; t += gridDim.x / sharing, ++turn) {
+            const bool more = walk.find(t);
+            const uint32_t i = turn & 1;
+            ok = __all_sync(0xffffffffu, bar_wait(tile_read + 8 * i, ((turn >> 1) & 1) ^ 1, gave_up));
+            if (!ok) break;
             if (lane == 0) {
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t s = it % STAGES, bar = full + 8 * s, at = smem_addr(ring) + s * S::kStageBytes;
-                    ok = bar_wait(empty + 8 * s, ((it / STAGES) & 1) ^ 1, gave_up);
-                    if (!ok) break;
-                    bar_expect(bar, S::kStageBytes);
-                    tma_load_3d(at, &wmap, bar, kb * kBlock, walk.n_tile * 128, walk.expert);
-                    tma_load_2d(at + 128 * kBlock, &xmap, bar, kb * kBlock, walk.row0);
+                tiles[i] = more ? make_int4(walk.expert, walk.row0, walk.row_end, walk.n_tile) : make_int4(-1, 0, 0, 0);
+                bar_arrive(tile_there + 8 * i);
+            }
+            if (!more) break;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t s = it % STAGES, at = smem_addr(ring) + s * S::kStageBytes;
+                const uint32_t bar = S::PAIR ? bar_at_rank(full + 8 * s, 0) : full + 8 * s;
+                ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, ((it / STAGES) & 1) ^ 1, gave_up));
+                if (!ok) break;
+                if (elect_one()) {
+                    if (half == 0) bar_expect(full + 8 * s, S::PAIR ? 2 * S::kStageBytes : S::kStageBytes);
+                    tma_load_3d<S::PAIR>(S::SWAP ? at : at + 128 * kBlock, &wmap, bar, kb * kBlock, walk.n_tile * S::kOutputs + int(half) * S::kRowsB, walk.expert);
+                    tma_load_2d<S::PAIR>(S::SWAP ? at + 128 * kBlock : at, &xmap, bar, kb * kBlock, walk.row0 + int(half) * 128);
                 }
             }
-            ok = __shfl_sync(0xffffffffu, int(ok), 0);
         }
         if (ok && lane == 0)  // every arrival at the ring's barriers has happened before the CTA ends
             for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) bar_wait(empty + 8 * (i % STAGES), (i / STAGES) & 1, gave_up);
         if (!ok && lane == 0)  // the copies in flight land before the CTA ends
             for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
                 const uint64_t t0 = global_ns();
-                while (!bar_try<false>(full + 8 * (i % STAGES), (i / STAGES) & 1) && global_ns() - t0 < kWaitLimitNs) {
+                while (!(half == 0 && bar_try<false>(full + 8 * (i % STAGES), (i / STAGES) & 1)) && global_ns() - t0 < kDrainLimitNs) {
                 }
             }
-    } else if (warp == 1) {  // ---- matrix instructions
+    } else if (warp == S::kIssue) {  // ---- matrix instructions
         uint32_t it = 0;
         bool ok = true;
-        for (int64_t t = first; ok && walk.find(t); t += step) {
-            if (lane == 0) {
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t s = it % STAGES, b = it % NBUF;
-                    ok = bar_wait(taken + 8 * b, ((it / NBUF) & 1) ^ 1, gave_up) && bar_wait(full + 8 * s, (it / STAGES) & 1, gave_up);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t at = smem_addr(ring) + s * S::kStageBytes;
-                    const uint64_t wd = tc_operand(at), xd = tc_operand(at + 128 * kBlock);
+        while (ok && next_tile()) {
+            if (half != 0) continue;
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const uint32_t s = it % STAGES, b = it % NBUF;
+                ok = __all_sync(0xffffffffu, bar_wait(taken + 8 * b, ((it / NBUF) & 1) ^ 1, gave_up) && bar_wait(full + 8 * s, (it / STAGES) & 1, gave_up));
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t at = smem_addr(ring) + s * S::kStageBytes;
+                const uint64_t ad = tc_operand(at), bd = tc_operand(at + 128 * kBlock);
+                if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8(tmem + b * BN, wd + 2 * k, xd + 2 * k, idesc, k > 0);
-                    tc_commit(empty + 8 * s);
-                    tc_commit(done + 8 * b);
+                    for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8<S::PAIR>(tmem + b * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0);
+                    tc_commit<S::PAIR>(empty + 8 * s);
+                    tc_commit<S::PAIR>(done + 8 * b);
                 }
             }
-            ok = __shfl_sync(0xffffffffu, int(ok), 0);
         }
-        if (!ok && lane == 0) {  // the instructions in flight end before their memory is given back
-            tc_commit(drained);
+        if (!ok && elect_one()) {  // the instructions in flight end before their memory is given back
+            tc_commit<S::PAIR>(drained);
             const uint64_t t0 = global_ns();
-            while (!bar_try<false>(drained, 0) && global_ns() - t0 < kWaitLimitNs) {
+            while (!bar_try<false>(drained, 0) && global_ns() - t0 < kDrainLimitNs) {
             }
         }
-    } else if (warp < 2 + S::kScaleWarps) {  // ---- scales, read four column blocks ahead
-        constexpr int kAhead = 4, kPer = S::kScalesPerLane;
-        const int col0 = (warp - 2) * (BN / S::kScaleWarps) + lane;
+    } else if (warp >= S::kScaling) {
+      if constexpr (S::SWAP) {  // ---- scales, read four column blocks ahead
+        constexpr int kPer = S::kScalesPerLane, kAhead = 4;
+        const int col0 = (warp - S::kScaling) * S::kScalesPerWarp + lane;  // columns col0 + 32 * i are this lane's
         uint32_t it = 0;
         bool ok = true;
-        for (int64_t t = first; ok && walk.find(t); t += step) {
-            const float* const sw = p.w.scales + walk.expert * p.w.sms + walk.n_tile * p.w.srs;
-            const float* const sx = p.x.scales + (walk.row0 + col0) * p.x.srs;
-            const int here = walk.row_end - walk.row0 - col0;  // column 32 * i of this lane exists if 32 * i < here
+        while (ok && next_tile()) {
+            const float* const sw = p.w.scales + tile.x * p.w.sms + tile.w * p.w.srs;
+            const int row = tile.y + col0;
+            const float* const sx = p.x.scales + row * p.x.srs;
+            const int here = tile.z - row;  // column 32 * i of this lane exists if 32 * i < here
             float x[kAhead][kPer], w[kAhead];
             auto load = [&](int kb) {
 #pragma unroll
@@ -250,46 +339,125 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                 }
             }
         }
-    } else if (warp >= 4) {  // ---- epilogue
-        constexpr int kCols = S::kCols;
-        const int quarter = warp & 3, col0 = (warp - 4) / 4 * kCols;
-        const uint32_t my_tmem = tmem + (uint32_t(quarter) << 21) + col0;
-        uint32_t it = 0, round = 0;
+      } else if (warp == S::kScaling) {  // ---- scales of kAhead column blocks into the next slot, by asynchronous copies
+        uint32_t chunk = 0;
         bool ok = true;
-        for (int64_t t = first; ok && walk.find(t); t += step) {
+        while (ok && next_tile()) {
+            const int row = tile.y + int(half) * 128 + lane;
+            const float* const sx = p.x.scales + row * p.x.srs;
+            const int64_t wb0 = int64_t(tile.w) * S::kOutputs / 128;
+            for (int kb = kb0; kb < kb1; kb += S::kAhead, ++chunk) {
+                const uint32_t slot = chunk % S::kSlots, at = smem_addr(scales) + slot * S::kSlotBytes;
+                ok = __all_sync(0xffffffffu, bar_wait(slot_read + 8 * slot, ((chunk / S::kSlots) & 1) ^ 1, gave_up));
+                if (!ok) break;
+#pragma unroll
+                for (int a = 0; a < S::kAhead; ++a)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const bool in = kb + a < kb1 && row + 32 * i < tile.z;
+                        copy_word_async(at + (a * 128 + 32 * i + lane) * 4, in ? sx + 32 * i * p.x.srs + (kb + a) * p.x.scs : p.x.scales, in);
+                    }
+                if (lane < 2 * S::kAhead) {
+                    const int a = lane % S::kAhead;
+                    const bool in = kb + a < kb1;
+                    const int64_t wb = min(wb0 + lane / S::kAhead, p.w.row_blocks - 1);
+                    copy_word_async(at + (S::kAhead * 128 + lane) * 4, in ? p.w.scales + tile.x * p.w.sms + wb * p.w.srs + (kb + a) * p.w.scs : p.w.scales, in);
+                }
+                bar_arrive_copies(slot_full + 8 * slot);
+            }
+        }
+        copies_wait_all();
+      }
+    }
+    } else {  // ---- epilogue
+        if constexpr (S::kTrades) regs_take<kTaken>();
+        constexpr int kCols = S::kCols;
+        const int quarter = warp & 3, col0 = warp / 4 * kCols;
+        const uint32_t my_tmem = tmem + (uint32_t(quarter) << 21) + col0;
+        uint32_t it = 0, round = 0, chunk = 0;
+        bool ok = true;
+        while (ok && next_tile()) {
             uint64_t acc[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t b = it % NBUF, ph = (it / NBUF) & 1;
-                ok = bar_wait(scaled + 8 * b, ph, gave_up) && bar_wait(done + 8 * b, ph, gave_up);
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                tc_fence_after();
-                const float* const sc = scales + b * BN + col0;
+            if constexpr (!S::SWAP) {
+                const float* const my_scale = scales + quarter * 32 + lane;
+                const float* const my_weight = scales + S::kAhead * 128 + col0 / 128 * S::kAhead;
+                // The waits' results are looked at once per tile: a warp that only goes on after all of its lanes have
+                // agreed lost 80 cycles per column block.
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const int a = (kb - kb0) % S::kAhead;
+                    const uint32_t slot = chunk % S::kSlots, b = it % NBUF;
+                    if (a == 0) bar_wait(slot_full + 8 * slot, (chunk / S::kSlots) & 1, gave_up);
+                    const uint32_t s1 = __float_as_uint(__fmul_rn(my_scale[slot * (S::kSlotBytes / 4) + a * 128], my_weight[slot * (S::kSlotBytes / 4) + a]));
+                    const uint64_t s2 = pack2(s1, s1);
+                    if (a == S::kAhead - 1 || kb + 1 == kb1) {
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(slot_read + 8 * slot);
+                        ++chunk;
+                    }
+                    bar_wait(done + 8 * b, (it / NBUF) & 1, gave_up);
+                    __syncwarp();
+                    tc_fence_after();
+                    uint32_t v[2][S::LOAD];  // one part being multiplied, the next one on its way
+                    tmem_load(v[0], my_tmem + b * BN);
 #pragma unroll
-                for (int c = 0; c < kCols; c += 16) {
-                    uint32_t v[16];
-                    tmem_load_16(v, my_tmem + b * BN + c);
-                    tmem_load_wait();
+                    for (int c = 0; c < kCols; c += S::LOAD) {
+                        uint32_t (&u)[S::LOAD] = v[c / S::LOAD & 1];
+                        tmem_load_wait(u);
+                        if (c + S::LOAD < kCols) tmem_load(v[(c / S::LOAD + 1) & 1], my_tmem + b * BN + c + S::LOAD);
+                        if (c + S::LOAD == kCols) {  // all of it is in registers: the accumulator may be written again
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) {
+                                if constexpr (S::PAIR) bar_arrive_remote(bar_at_rank(taken + 8 * b, 0));
+                                else bar_arrive(taken + 8 * b);
+                            }
+                        }
 #pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const uint4 s4 = *reinterpret_cast<const uint4*>(sc + c + i);
-                        fma2(acc[(c + i) / 2], pack2(v[i], v[i + 1]), pack2(s4.x, s4.y));
-                        fma2(acc[(c + i) / 2 + 1], pack2(v[i + 2], v[i + 3]), pack2(s4.z, s4.w));
+                        for (int i = 0; i < S::LOAD; i += 2) fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), s2);
                     }
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) bar_arrive(taken + 8 * b);
+                ok = !__any_sync(0xffffffffu, *gave_up);
+            } else {
+                for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                    const uint32_t b = it % NBUF, ph = (it / NBUF) & 1;
+                    ok = bar_wait(scaled + 8 * b, ph, gave_up) && bar_wait(done + 8 * b, ph, gave_up);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const float* const sc = scales + b * BN + col0;
+#pragma unroll
+                    for (int c = 0; c < kCols; c += 16) {
+                        uint32_t v[16];
+                        tmem_load(v, my_tmem + b * BN + c);
+                        tmem_load_wait(v);
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const uint4 s4 = *reinterpret_cast<const uint4*>(sc + c + i);
+                            fma2(acc[(c + i) / 2], pack2(v[i], v[i + 1]), pack2(s4.x, s4.y));
+                            fma2(acc[(c + i) / 2 + 1], pack2(v[i + 2], v[i + 3]), pack2(s4.z, s4.w));
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(taken + 8 * b);
+                }
             }
             if (!ok) break;
-            const int here = walk.row_end - walk.row0;
-            const int n = walk.n_tile * 128 + quarter * 32 + lane;
-            T* const out = static_cast<T*>(p.out) + int64_t(walk.row0) * p.out_ld + n;
+            const int here = tile.z - tile.y;
+            if constexpr (!S::SWAP) {
+                const int m = tile.y + int(half) * 128 + quarter * 32, n = tile.w * S::kOutputs + col0;
+                if (m < tile.z && n < p.w.rows)
+                    store_rows<T, kCols>(extra + warp * 4096, static_cast<T*>(p.out) + m * p.out_ld + n, p.out_ld, acc, min(32, tile.z - m),
+                                         int(min(int64_t(kCols), p.w.rows - n)), lane);
+                continue;
+            }
+            const int n = tile.w * 128 + quarter * 32 + lane;
+            T* const out = static_cast<T*>(p.out) + int64_t(tile.y) * p.out_ld + n;
             if (S::kSplits && ranks > 1) {
                 if constexpr (S::kSplits) {
-                    float* const mine = partial + quarter * 32 + lane;
+                    float* const mine = reinterpret_cast<float*>(extra) + quarter * 32 + lane;
                     ok = __all_sync(0xffffffffu, bar_wait<true>(parts_free, (round & 1) ^ 1, gave_up));
                     if (!ok) break;
 #pragma unroll
@@ -319,10 +487,11 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == 2) tmem_free(tmem, S::kTmem);
+    if (S::PAIR) cluster_sync();  // both CTAs have read their accumulators
+    if (warp == S::kIssue) tmem_free<S::PAIR>(tmem, S::kTmem);
     if (threadIdx.x == 0 && *gave_up) set_flag(flags, VF_FLAG_GAVE_UP);
     __syncwarp();
-    if (ranks > 1) cluster_sync();  // no CTA ends while another one reads its sums
+    if (in_cluster) cluster_sync();  // no CTA ends while another one reads its sums
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -357,11 +526,17 @@ bool fits_bulk_copies(const Blocks& b) {  // start and pitches of 16-byte units,
 }
 
 template <class S, class T>
-void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks) {
+void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
+    if (S::PAIR) ranks = 2;
     auto kernel = k_matmul_blocks<S, T>;
     VF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    const int64_t n_tiles = (p.w.rows + 127) / 128;
-    const int64_t tiles = most_row_tiles(p, S::BN) * n_tiles;
+    if (S::kTrades) {  // warps that take registers wait until they are there: what is taken has to have been given
+        cudaFuncAttributes fa;
+        VF_CUDA(cudaFuncGetAttributes(&fa, kernel));
+        if (fa.numRegs * S::kThreads < 128 * kGiven + 128 * S::GROUPS * kTaken) raise(VF_ERR_CUDA, "the kernel was built with too few registers");
+    }
+    const int64_t n_tiles = (p.w.rows + S::kOutputs - 1) / S::kOutputs;
+    const int64_t tiles = most_row_tiles(p, S::kTokens) * n_tiles;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(std::min<int64_t>(tiles, std::max(1, ctx->sm_count * S::PER_SM / ranks)) * ranks));
     cfg.blockDim = dim3(S::kThreads);
@@ -373,16 +548,17 @@ void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks) {
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    const uint32_t idesc = tc_f8_shape(p.w.dtype == VF_DT_F8E5M2, p.x.dtype == VF_DT_F8E5M2, S::BN);
-    VF_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_codes(p.x, 2, S::BN), map_codes(p.w, 3, 128), p, int(n_tiles), idesc, ctx->d_flags));
+    const uint32_t idesc = tc_f8_shape((S::SWAP ? p.w : p.x).dtype == VF_DT_F8E5M2, (S::SWAP ? p.x : p.w).dtype == VF_DT_F8E5M2, S::PAIR ? 256 : 128, S::BN);
+    VF_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_codes(p.x, 2, S::PAIR ? 128 : S::kTokens), map_codes(p.w, 3, S::SWAP ? 128 : S::kRowsB), p, int(n_tiles), idesc, ctx->d_flags));
 }
 
-//                     BN, stages, accumulators, epilogue groups of four warps, CTAs per SM
-using Shape16 = Shape<16, 5, 4, 1, 2>;
-using Shape32 = Shape<32, 4, 4, 1, 2>;
-using Shape64 = Shape<64, 4, 4, 1, 2>;
-using Shape128 = Shape<128, 6, 2, 2, 1>;
-using Shape256 = Shape<256, 4, 2, 4, 1>;
+//                       BN, stages, accumulators, epilogue groups of four warps, CTAs per SM
+using Swap16 = Shape<Form::kSwap, 16, 5, 4, 1, 2>;
+using Swap32 = Shape<Form::kSwap, 32, 4, 4, 1, 2>;
+using Swap64 = Shape<Form::kSwap, 64, 4, 4, 1, 2>;
+using Single64 = Shape<Form::kSingle, 64, 3, 4, 1, 2>;
+using Single128 = Shape<Form::kSingle, 128, 5, 2, 2, 1>;
+using Pair256 = Shape<Form::kPair, 256, 5, 2, 2, 1, 16>;
 
 template <class T>
 void launch_for(vf_ctx* ctx, const BlockProduct& p) {
@@ -394,14 +570,14 @@ void launch_for(vf_ctx* ctx, const BlockProduct& p) {
         const int64_t tiles = most_row_tiles(p, bn) * n_tiles;
         int ranks = 1;
         while (ranks < 8 && tiles * ranks * 2 <= 2 * ctx->sm_count && p.x.col_blocks >= 4 * ranks) ranks *= 2;
-        if (bn == 16) launch_tensor<Shape16, T>(ctx, p, ranks);
-        else launch_tensor<Shape32, T>(ctx, p, ranks);
+        if (bn == 16) launch_tensor<Swap16, T>(ctx, p, ranks);
+        else launch_tensor<Swap32, T>(ctx, p, ranks);
     } else if (rows <= 64) {
-        launch_tensor<Shape64, T>(ctx, p, 1);
-    } else if (rows <= 128) {
-        launch_tensor<Shape128, T>(ctx, p, 1);
+        launch_tensor<Swap64, T>(ctx, p);
     } else {
-        launch_tensor<Shape256, T>(ctx, p, 1);
+        if (most_row_tiles(p, 256) * ((p.w.rows + 255) / 256) >= ctx->sm_count / 2) launch_tensor<Pair256, T>(ctx, p);
+        else if (most_row_tiles(p, 128) * n_tiles >= ctx->sm_count) launch_tensor<Single128, T>(ctx, p);
+        else launch_tensor<Single64, T>(ctx, p);
     }
 }
 

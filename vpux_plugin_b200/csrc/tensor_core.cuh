@@ -13,6 +13,14 @@ __device__ __forceinline__ uint32_t smem_addr(const void* p) {
     return uint32_t(__cvta_generic_to_shared(p));
 }
 
+// true in one thread of the (converged) warp. Branching on this and not on the lane number keeps the branch's operands in
+// uniform registers, where the tensor-core and bulk-copy instructions want them.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p)::"memory");
+    return p != 0;
+}
+
 // ---- mbarriers -----------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -32,6 +40,16 @@ __device__ __forceinline__ void bar_arrive_at(uint32_t bar, uint32_t rank) {
         "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar),
         "r"(rank)
         : "memory");
+}
+__device__ __forceinline__ uint32_t bar_at_rank(uint32_t bar, uint32_t rank) {  // the same barrier of another CTA of the cluster
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(bar), "r"(rank));
+    return a;
+}
+// arrives at the barrier with the cluster address `bar`, for what tensor memory holds: no writes of this thread have to be
+// visible to the other CTA (a release to the whole cluster waits for all of them and took a microsecond)
+__device__ __forceinline__ void bar_arrive_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 template <bool Cluster>
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
@@ -55,11 +73,12 @@ __device__ __forceinline__ uint64_t global_ns() {
 }
 
 constexpr uint64_t kWaitLimitNs = 4000000000ull;  // no wait of these kernels lasts longer than microseconds
+constexpr uint64_t kDrainLimitNs = 1000000;    // and after one gave up, copies and instructions in flight end within this
 
 // Waits until the phase `parity` of the barrier is complete. Gives up after the time limit, or when another thread of the
 // CTA has: `gave_up` (shared memory) is then set and false is returned.
 template <bool Cluster = false>
-__device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+__device__ __forceinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
     const uint64_t t0 = global_ns();
     for (;;) {
         for (int i = 0; i < 64; ++i)
@@ -73,7 +92,7 @@ __device__ __noinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volati
 }
 template <bool Cluster = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 1024; ++i)  // (reading the clock would delay a wait that is about to end)
         if (bar_try<Cluster>(bar, parity)) return true;
     return bar_wait_long<Cluster>(bar, parity, gave_up);
 }
@@ -98,28 +117,63 @@ __device__ __forceinline__ float load_from_rank(uint32_t addr, uint32_t rank) {
     return v;
 }
 
+// ---- asynchronous copies of single words -------------------------------------------------------------------------------
+// `in` false: reads nothing and writes zero
+__device__ __forceinline__ void copy_word_async(uint32_t dst, const float* src, bool in) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(in ? 4 : 0) : "memory");
+}
+// this thread's arrival at `bar`, when its copies so far have landed
+__device__ __forceinline__ void bar_arrive_copies(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
 // ---- bulk tensor copies ----------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }
+// `bar` belongs to this CTA, or (Pair) to either CTA of the pair: an address from bar_at_rank()
+template <bool Pair>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m), "r"(bar),
-                 "r"(x), "r"(y)
-                 : "memory");
+    if constexpr (Pair)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+                     "l"(m), "r"(bar), "r"(x), "r"(y)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m), "r"(bar),
+                     "r"(x), "r"(y)
+                     : "memory");
 }
+template <bool Pair>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(m),
-                 "r"(bar), "r"(x), "r"(y), "r"(z)
-                 : "memory");
+    if constexpr (Pair)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+                     "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(m),
+                     "r"(bar), "r"(x), "r"(y), "r"(z)
+                     : "memory");
 }
 
 // ---- tensor core -------------------------------------------------------------------------------------------------------
+// Pair: the two CTAs of a pair (cluster ranks 2i and 2i + 1) work on one tile. Both allocate and free, the even one issues.
+template <bool Pair>
 __device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t columns) {  // one whole warp
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (Pair) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
 }
+template <bool Pair>
 __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {  // the warp that allocated
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
+    if constexpr (Pair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -127,28 +181,41 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// arrives at `bar` once every tensor-core operation that this thread has issued is complete
+// arrives at `bar` (Pair: of both CTAs) once every tensor-core operation that this thread has issued is complete
+template <bool Pair>
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (Pair)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3))
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// D[128 x N] (+)= A[128 x 32] * B[N x 32]^T, 8-bit floats in shared memory, fp32 in tensor memory
+// D[128 x N] (+)= A[128 x 32] * B[N x 32]^T, 8-bit floats in shared memory, fp32 in tensor memory. Pair: D and A have 256 rows,
+// 128 in each CTA, and each CTA holds half of B's rows.
+template <bool Pair>
 __device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"(uint32_t(accumulate))
-        : "memory");
+    if constexpr (Pair)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+            "r"(idesc), "r"(uint32_t(accumulate))
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+            "r"(idesc), "r"(uint32_t(accumulate))
+            : "memory");
 }
 // Descriptor of an operand tile in shared memory: rows of 128 bytes (K contiguous) in the 128-byte swizzle that the bulk copies
 // write, groups of eight rows 1024 bytes apart. The start address moves by 32 bytes per step of 32 k.
 __device__ __forceinline__ uint64_t tc_operand(uint32_t addr) {
     return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
-// Instruction descriptor of kind::f8f6f4: fp32 result, both operands K-major, M = 128
-__host__ __device__ inline uint32_t tc_f8_shape(bool a_e5m2, bool b_e5m2, int n) {
-    return (1u << 4) | (uint32_t(a_e5m2) << 7) | (uint32_t(b_e5m2) << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+// Instruction descriptor of kind::f8f6f4: fp32 result, both operands K-major
+__host__ __device__ inline uint32_t tc_f8_shape(bool a_e5m2, bool b_e5m2, int m, int n) {
+    return (1u << 4) | (uint32_t(a_e5m2) << 7) | (uint32_t(b_e5m2) << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 // 16 consecutive columns of this warp's 32 lanes (one lane per thread)
-__device__ __forceinline__ void tmem_load_16(uint32_t (&v)[16], uint32_t addr) {
+__device__ __forceinline__ void tmem_load(uint32_t (&v)[16], uint32_t addr) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
         : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
@@ -156,8 +223,22 @@ __device__ __forceinline__ void tmem_load_16(uint32_t (&v)[16], uint32_t addr) {
         : "r"(addr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_load_wait() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+__device__ __forceinline__ void tmem_load(uint32_t (&v)[32], uint32_t addr) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
+        "%23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+          "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]),
+          "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr)
+        : "memory");
+}
+// Waits for every load of this thread; `v` passes through, so that no use of the loaded values moves in front of the wait
+__device__ __forceinline__ void tmem_load_wait(uint32_t (&v)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])::"memory");
+}
+__device__ __forceinline__ void tmem_load_wait(uint32_t (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]), "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]), "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])::"memory");
 }
 
 // ---- packed fp32 pairs -------------------------------------------------------------------------------------------------
@@ -168,6 +249,16 @@ __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
 }
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+// Registers of a whole group of four warps: what some give up others may take, up to what the block was launched with
+template <int R>
+__device__ __forceinline__ void regs_give() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_take() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
 }
 
 }  // namespace vf
