@@ -104,22 +104,21 @@ struct Shape {
     static constexpr int BN = BN_, STAGES = STAGES_, NBUF = NBUF_, GROUPS = GROUPS_, PER_SM = PER_SM_, LOAD = LOAD_;
     static constexpr int kCols = BN / GROUPS;               // columns of the accumulator per epilogue warp
     static constexpr int kTokens = SWAP ? BN : (PAIR ? 256 : 128), kOutputs = SWAP ? 128 : BN;  // a tile's results
-    static constexpr int kScaleWarps = SWAP && BN >= 64 ? 2 : 1;
     static constexpr int kEpilogue = 4 * GROUPS, kCopies = kEpilogue, kIssue = kEpilogue + 1, kScaling = kEpilogue + 2;  // warps
     static constexpr bool kTrades = kCols > 64;             // the warps behind the epilogue's give it registers, as a group of four
-    static constexpr int kThreads = 32 * (kEpilogue + (kTrades ? 4 : 2 + kScaleWarps));
-    // activations as the 128-row operand: scales of kAhead column blocks at a time, [kAhead][128] of rows, [2][kAhead] of weights
-    static constexpr int kAhead = 8, kSlots = 2, kSlotBytes = kAhead * 128 * 4 + 2 * kAhead * 4;
-    static constexpr int kScalesPerWarp = BN / kScaleWarps;
-    static constexpr int kScalesPerLane = (kScalesPerWarp + 31) / 32;
+    static constexpr int kThreads = 32 * (kEpilogue + (kTrades ? 4 : 3));
+    // scales of kAhead column blocks at a time: [kAhead][kTileRows] of the activations, [kTileBlocks][kAhead] of the weights
+    static constexpr int kAhead = 8, kSlots = 2, kTileRows = SWAP ? BN : 128, kTileBlocks = SWAP ? 1 : 2;
+    static constexpr int kSlotBytes = kAhead * (kTileRows + kTileBlocks) * 4;
     static constexpr int kRowsB = PAIR ? BN / 2 : BN;       // rows of the second operand that this CTA holds
     static constexpr int kStageBytes = (128 + kRowsB) * kBlock;
     static constexpr int kTmem = NBUF * BN < 32 ? 32 : NBUF * BN;
-    static constexpr bool kSplits = SWAP && BN <= 32;       // clusters share a tile's column blocks
+    // clusters share a tile's column blocks: four columns of a tile at a time, the CTAs of a cluster own them in turn
+    static constexpr int kFours = BN / 4, kParts = BN == 16 ? 8 : (BN == 32 ? 10 : 16);
     static constexpr int kRing = STAGES * kStageBytes;
-    static constexpr int kScales = SWAP ? NBUF * BN * 4 : kSlots * kSlotBytes;
-    static constexpr int kExtra = kSplits ? 128 * BN * 4 : (SWAP ? 0 : 4 * GROUPS * 4096);  // partial sums; results on their way out
-    static constexpr int kBars = 2 * STAGES + 3 * NBUF + 3 + 2 * 2 + 2 * kSlots;
+    static constexpr int kScales = kSlots * kSlotBytes;
+    static constexpr int kExtra = SWAP ? kParts * 128 * 16 : 4 * GROUPS * 4096;  // partial sums; results on their way out
+    static constexpr int kBars = 2 * STAGES + 2 * NBUF + 2 + 2 * 2 + 2 * kSlots;
     static constexpr int kSmem = 1024 + kRing + kScales + kExtra + 2 * 16 + kBars * 8 + 16;
 };
 
@@ -174,13 +173,13 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     uint32_t* const tmem_at = reinterpret_cast<uint32_t*>(bars + S::kBars);
     volatile int* const gave_up = reinterpret_cast<volatile int*>(tmem_at + 1);
     const uint32_t full = smem_addr(bars), empty = full + 8 * STAGES;                      // ring
-    const uint32_t done = empty + 8 * STAGES, scaled = done + 8 * NBUF, taken = scaled + 8 * NBUF;  // accumulators
-    const uint32_t parts_full = taken + 8 * NBUF, parts_free = parts_full + 8, drained = parts_free + 8;
+    const uint32_t done = empty + 8 * STAGES, taken = done + 8 * NBUF;                     // accumulators
+    const uint32_t parts_full = taken + 8 * NBUF, drained = parts_full + 8;
     const uint32_t tile_there = drained + 8, tile_read = tile_there + 16;
     const uint32_t slot_full = tile_read + 16, slot_read = slot_full + 8 * S::kSlots;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t ranks = S::kSplits ? cluster_size() : 1, rank = S::kSplits ? cluster_rank() : 0;  // CTAs that share a tile's column blocks
+    const uint32_t ranks = S::SWAP ? cluster_size() : 1, rank = S::SWAP ? cluster_rank() : 0;  // CTAs that share a tile's column blocks
     const uint32_t half = S::PAIR ? cluster_rank() : 0;
     const bool in_cluster = S::PAIR || ranks > 1;
     if (threadIdx.x == 0) {
@@ -190,15 +189,13 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         }
         for (int i = 0; i < NBUF; ++i) {
             bar_init(done + 8 * i, 1);
-            bar_init(scaled + 8 * i, S::kScaleWarps);
             bar_init(taken + 8 * i, (S::PAIR ? 8 : 4) * S::GROUPS);
         }
-        bar_init(parts_full, 4 * ranks);
-        bar_init(parts_free, 4 * ranks);
+        bar_init(parts_full, 1);
         bar_init(drained, 1);
         for (int i = 0; i < 2; ++i) {
             bar_init(tile_there + 8 * i, 1);
-            bar_init(tile_read + 8 * i, S::kEpilogue + 1 + S::kScaleWarps);
+            bar_init(tile_read + 8 * i, S::kEpilogue + 2);
         }
         for (int i = 0; i < S::kSlots; ++i) {
             bar_init(slot_full + 8 * i, 32);
@@ -212,9 +209,12 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     if (warp == S::kIssue) tmem_alloc<S::PAIR>(smem_addr(tmem_at), S::kTmem);
     tc_fence_before();
     __syncthreads();
-    if (in_cluster) cluster_sync();
+    if (S::PAIR) cluster_sync();
+    else if (in_cluster) cluster_arrive();  // waited for before anything goes to another CTA
+    bool joined = !in_cluster, left = !in_cluster;
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
+    chain_enter();  // set up while the kernel before this one was ending; from here on its results are read
 
     const int kbs = int(p.x.col_blocks), kb0 = int(rank * uint32_t(kbs) / ranks), kb1 = int((rank + 1) * uint32_t(kbs) / ranks);
     // The next tile, as the copying warp has found it; by whole warps
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         if (!ok && lane == 0)  // the copies in flight land before the CTA ends
             for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
                 const uint64_t t0 = global_ns();
-                while (!(half == 0 && bar_try<false>(full + 8 * (i % STAGES), (i / STAGES) & 1)) && global_ns() - t0 < kDrainLimitNs) {
+                while (!(half == 0 && bar_try(full + 8 * (i % STAGES), (i / STAGES) & 1)) && global_ns() - t0 < kDrainLimitNs) {
                 }
             }
     } else if (warp == S::kIssue) {  // ---- matrix instructions
@@ -291,55 +291,10 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         if (!ok && elect_one()) {  // the instructions in flight end before their memory is given back
             tc_commit<S::PAIR>(drained);
             const uint64_t t0 = global_ns();
-            while (!bar_try<false>(drained, 0) && global_ns() - t0 < kDrainLimitNs) {
+            while (!bar_try(drained, 0) && global_ns() - t0 < kDrainLimitNs) {
             }
         }
-    } else if (warp >= S::kScaling) {
-      if constexpr (S::SWAP) {  // ---- scales, read four column blocks ahead
-        constexpr int kPer = S::kScalesPerLane, kAhead = 4;
-        const int col0 = (warp - S::kScaling) * S::kScalesPerWarp + lane;  // columns col0 + 32 * i are this lane's
-        uint32_t it = 0;
-        bool ok = true;
-        while (ok && next_tile()) {
-            const float* const sw = p.w.scales + tile.x * p.w.sms + tile.w * p.w.srs;
-            const int row = tile.y + col0;
-            const float* const sx = p.x.scales + row * p.x.srs;
-            const int here = tile.z - row;  // column 32 * i of this lane exists if 32 * i < here
-            float x[kAhead][kPer], w[kAhead];
-            auto load = [&](int kb) {
-#pragma unroll
-                for (int a = 0; a < kAhead; ++a) {
-                    const bool in = kb + a < kb1;
-                    w[a] = in ? sw[(kb + a) * p.w.scs] : 0.f;
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) x[a][i] = in && 32 * i < here && col0 + 32 * i < BN ? sx[32 * i * p.x.srs + (kb + a) * p.x.scs] : 0.f;
-                }
-            };
-            load(kb0);
-            for (int kb = kb0; ok && kb < kb1; kb += kAhead) {
-                float v[kAhead][kPer];
-#pragma unroll
-                for (int a = 0; a < kAhead; ++a)
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) v[a][i] = __fmul_rn(x[a][i], w[a]);
-                if (kb + kAhead < kb1) load(kb + kAhead);
-#pragma unroll
-                for (int a = 0; a < kAhead; ++a) {
-                    if (kb + a >= kb1 || !ok) break;
-                    const uint32_t b = it % NBUF;
-                    ok = bar_wait(taken + 8 * b, ((it / NBUF) & 1) ^ 1, gave_up);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i)
-                        if (col0 + 32 * i < BN) scales[b * BN + col0 + 32 * i] = v[a][i];
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(scaled + 8 * b);
-                    ++it;
-                }
-            }
-        }
-      } else if (warp == S::kScaling) {  // ---- scales of kAhead column blocks into the next slot, by asynchronous copies
+    } else if (warp == S::kScaling) {  // ---- scales of kAhead column blocks into the next slot, by asynchronous copies
         uint32_t chunk = 0;
         bool ok = true;
         while (ok && next_tile()) {
@@ -353,97 +308,87 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
 #pragma unroll
                 for (int a = 0; a < S::kAhead; ++a)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < (S::kTileRows + 31) / 32; ++i) {
+                        if (S::kTileRows < 32 && lane >= S::kTileRows) break;
                         const bool in = kb + a < kb1 && row + 32 * i < tile.z;
-                        copy_word_async(at + (a * 128 + 32 * i + lane) * 4, in ? sx + 32 * i * p.x.srs + (kb + a) * p.x.scs : p.x.scales, in);
+                        copy_word_async(at + (a * S::kTileRows + 32 * i + lane) * 4, in ? sx + 32 * i * p.x.srs + (kb + a) * p.x.scs : p.x.scales, in);
                     }
-                if (lane < 2 * S::kAhead) {
+                if (lane < S::kTileBlocks * S::kAhead) {
                     const int a = lane % S::kAhead;
                     const bool in = kb + a < kb1;
                     const int64_t wb = min(wb0 + lane / S::kAhead, p.w.row_blocks - 1);
-                    copy_word_async(at + (S::kAhead * 128 + lane) * 4, in ? p.w.scales + tile.x * p.w.sms + wb * p.w.srs + (kb + a) * p.w.scs : p.w.scales, in);
+                    copy_word_async(at + (S::kAhead * S::kTileRows + lane) * 4, in ? p.w.scales + tile.x * p.w.sms + wb * p.w.srs + (kb + a) * p.w.scs : p.w.scales, in);
                 }
                 bar_arrive_copies(slot_full + 8 * slot);
             }
         }
         copies_wait_all();
-      }
     }
     } else {  // ---- epilogue
         if constexpr (S::kTrades) regs_take<kTaken>();
         constexpr int kCols = S::kCols;
         const int quarter = warp & 3, col0 = warp / 4 * kCols;
         const uint32_t my_tmem = tmem + (uint32_t(quarter) << 21) + col0;
-        uint32_t it = 0, round = 0, chunk = 0;
+        uint32_t it = 0, chunk = 0;
         bool ok = true;
         while (ok && next_tile()) {
             uint64_t acc[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
-            if constexpr (!S::SWAP) {
-                const float* const my_scale = scales + quarter * 32 + lane;
-                const float* const my_weight = scales + S::kAhead * 128 + col0 / 128 * S::kAhead;
-                // The waits' results are looked at once per tile: a warp that only goes on after all of its lanes have
-                // agreed lost 80 cycles per column block.
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const int a = (kb - kb0) % S::kAhead;
-                    const uint32_t slot = chunk % S::kSlots, b = it % NBUF;
-                    if (a == 0) bar_wait(slot_full + 8 * slot, (chunk / S::kSlots) & 1, gave_up);
-                    const uint32_t s1 = __float_as_uint(__fmul_rn(my_scale[slot * (S::kSlotBytes / 4) + a * 128], my_weight[slot * (S::kSlotBytes / 4) + a]));
-                    const uint64_t s2 = pack2(s1, s1);
-                    if (a == S::kAhead - 1 || kb + 1 == kb1) {
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(slot_read + 8 * slot);
-                        ++chunk;
-                    }
-                    bar_wait(done + 8 * b, (it / NBUF) & 1, gave_up);
+            const float* const my_scale = scales + (S::SWAP ? col0 : quarter * 32 + lane);
+            const float* const my_weight = scales + S::kAhead * S::kTileRows + (S::SWAP ? 0 : col0 / 128 * S::kAhead);
+            // The waits' results are looked at once per tile: a warp that only goes on after all of its lanes have agreed
+            // lost 80 cycles per column block.
+            for (int kb = kb0; kb < kb1; ++kb, ++it) {
+                const int a = (kb - kb0) % S::kAhead;
+                const uint32_t slot = chunk % S::kSlots, b = it % NBUF;
+                if (a == 0) bar_wait(slot_full + 8 * slot, (chunk / S::kSlots) & 1, gave_up);
+                const float* const sx = my_scale + slot * (S::kSlotBytes / 4) + a * S::kTileRows;
+                float scale = my_weight[slot * (S::kSlotBytes / 4) + a];
+                if (!S::SWAP) scale = __fmul_rn(*sx, scale);
+                const uint64_t s2 = pack2(__float_as_uint(scale), __float_as_uint(scale));
+                const bool last = a == S::kAhead - 1 || kb + 1 == kb1;  // of its slot
+                if (!S::SWAP && last) {
                     __syncwarp();
-                    tc_fence_after();
-                    uint32_t v[2][S::LOAD];  // one part being multiplied, the next one on its way
-                    tmem_load(v[0], my_tmem + b * BN);
+                    if (lane == 0) bar_arrive(slot_read + 8 * slot);
+                }
+                bar_wait(done + 8 * b, (it / NBUF) & 1, gave_up);
+                __syncwarp();
+                tc_fence_after();
+                uint32_t v[2][S::LOAD];  // one part being multiplied, the next one on its way
+                tmem_load(v[0], my_tmem + b * BN);
 #pragma unroll
-                    for (int c = 0; c < kCols; c += S::LOAD) {
-                        uint32_t (&u)[S::LOAD] = v[c / S::LOAD & 1];
-                        tmem_load_wait(u);
-                        if (c + S::LOAD < kCols) tmem_load(v[(c / S::LOAD + 1) & 1], my_tmem + b * BN + c + S::LOAD);
-                        if (c + S::LOAD == kCols) {  // all of it is in registers: the accumulator may be written again
-                            tc_fence_before();
-                            __syncwarp();
-                            if (lane == 0) {
-                                if constexpr (S::PAIR) bar_arrive_remote(bar_at_rank(taken + 8 * b, 0));
-                                else bar_arrive(taken + 8 * b);
-                            }
+                for (int c = 0; c < kCols; c += S::LOAD) {
+                    uint32_t(&u)[S::LOAD] = v[c / S::LOAD & 1];
+                    tmem_load_wait(u);
+                    if (c + S::LOAD < kCols) tmem_load(v[(c / S::LOAD + 1) & 1], my_tmem + b * BN + c + S::LOAD);
+                    if (c + S::LOAD == kCols) {  // all of it is in registers: the accumulator may be written again
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if constexpr (S::PAIR) bar_arrive_remote(bar_at_rank(taken + 8 * b, 0));
+                            else bar_arrive(taken + 8 * b);
                         }
+                    }
+                    if constexpr (S::SWAP) {
+#pragma unroll
+                        for (int i = 0; i < S::LOAD; i += 4) {
+                            const uint4 s4 = *reinterpret_cast<const uint4*>(sx + c + i);
+                            fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), mul2(pack2(s4.x, s4.y), s2));
+                            fma2(acc[(c + i) / 2 + 1], pack2(u[i + 2], u[i + 3]), mul2(pack2(s4.z, s4.w), s2));
+                        }
+                    } else {
 #pragma unroll
                         for (int i = 0; i < S::LOAD; i += 2) fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), s2);
                     }
                 }
-                ok = !__any_sync(0xffffffffu, *gave_up);
-            } else {
-                for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                    const uint32_t b = it % NBUF, ph = (it / NBUF) & 1;
-                    ok = bar_wait(scaled + 8 * b, ph, gave_up) && bar_wait(done + 8 * b, ph, gave_up);
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const float* const sc = scales + b * BN + col0;
-#pragma unroll
-                    for (int c = 0; c < kCols; c += 16) {
-                        uint32_t v[16];
-                        tmem_load(v, my_tmem + b * BN + c);
-                        tmem_load_wait(v);
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const uint4 s4 = *reinterpret_cast<const uint4*>(sc + c + i);
-                            fma2(acc[(c + i) / 2], pack2(v[i], v[i + 1]), pack2(s4.x, s4.y));
-                            fma2(acc[(c + i) / 2 + 1], pack2(v[i + 2], v[i + 3]), pack2(s4.z, s4.w));
-                        }
-                    }
-                    tc_fence_before();
+                if (S::SWAP && last) {
                     __syncwarp();
-                    if (lane == 0) bar_arrive(taken + 8 * b);
+                    if (lane == 0) bar_arrive(slot_read + 8 * slot);
                 }
+                if (last) ++chunk;
             }
+            ok = !__any_sync(0xffffffffu, *gave_up);
             if (!ok) break;
             const int here = tile.z - tile.y;
             if constexpr (!S::SWAP) {
@@ -455,26 +400,45 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
             }
             const int n = tile.w * 128 + quarter * 32 + lane;
             T* const out = static_cast<T*>(p.out) + int64_t(tile.y) * p.out_ld + n;
-            if (S::kSplits && ranks > 1) {
-                if constexpr (S::kSplits) {
-                    float* const mine = reinterpret_cast<float*>(extra) + quarter * 32 + lane;
-                    ok = __all_sync(0xffffffffu, bar_wait<true>(parts_free, (round & 1) ^ 1, gave_up));
-                    if (!ok) break;
+            if (S::SWAP && ranks > 1) {
+                // Four columns go to the CTA that owns them, which has a place for every rank's; the only tile of this
+                // cluster, so nobody has to be asked whether a place is free.
+                if constexpr (S::SWAP) {
+                    const int fours = (min(here, BN) + 3) / 4, mine = fours > int(rank) ? (fours - int(rank) - 1) / int(ranks) + 1 : 0;
+                    const int places = (S::kFours + int(ranks) - 1) / int(ranks);
+                    if (threadIdx.x == 0 && mine) bar_expect(parts_full, mine * int(ranks) * 128 * 16);
+                    __syncwarp();
+                    cluster_wait();
+                    joined = true;
+                    const uint32_t my_place = smem_addr(extra) + (rank * places * 128 + quarter * 32 + lane) * 16;
 #pragma unroll
-                    for (int i = 0; i < kCols; ++i)
-                        if (i < here) mine[i * 128] = __uint_as_float(uint32_t(acc[i / 2] >> (32 * (i & 1))));
+                    for (int g = 0; g < S::kFours; ++g)
+                        if (g < fours)
+                            push_to_rank(my_place + g / int(ranks) * 128 * 16, parts_full, g % int(ranks), uint32_t(acc[2 * g]), uint32_t(acc[2 * g] >> 32),
+                                         uint32_t(acc[2 * g + 1]), uint32_t(acc[2 * g + 1] >> 32));
                     __syncwarp();
-                    if (lane < ranks) bar_arrive_at(parts_full, lane);
-                    ok = __all_sync(0xffffffffu, bar_wait<true>(parts_full, round & 1, gave_up));
+                    cluster_arrive_relaxed();
+                    left = true;
+                    if (!mine) continue;
+                    ok = __all_sync(0xffffffffu, bar_wait(parts_full, 0, gave_up));
                     if (!ok) break;
-                    for (int i = int(rank); i < here && i < BN; i += int(ranks)) {
-                        float v = 0.f;
-                        for (uint32_t r = 0; r < ranks; ++r) v = __fadd_rn(v, load_from_rank(smem_addr(mine + i * 128), r));
-                        if (n < p.w.rows) out[i * p.out_ld] = to_wide<T>(v);
+                    const float4* const parts = reinterpret_cast<const float4*>(extra) + quarter * 32 + lane;
+                    for (int j = 0; j < mine; ++j) {
+                        float4 v = parts[j * 128];
+                        for (int r = 1; r < int(ranks); ++r) {
+                            const float4 q = parts[(r * places + j) * 128];
+                            v.x = __fadd_rn(v.x, q.x);
+                            v.y = __fadd_rn(v.y, q.y);
+                            v.z = __fadd_rn(v.z, q.z);
+                            v.w = __fadd_rn(v.w, q.w);
+                        }
+                        const int i = 4 * (int(rank) + j * int(ranks));
+                        if (n >= p.w.rows) continue;
+                        out[int64_t(i) * p.out_ld] = to_wide<T>(v.x);
+                        if (i + 1 < here) out[int64_t(i + 1) * p.out_ld] = to_wide<T>(v.y);
+                        if (i + 2 < here) out[int64_t(i + 2) * p.out_ld] = to_wide<T>(v.z);
+                        if (i + 3 < here) out[int64_t(i + 3) * p.out_ld] = to_wide<T>(v.w);
                     }
-                    __syncwarp();
-                    if (lane < ranks) bar_arrive_at(parts_free, lane);
-                    ++round;
                 }
             } else if (n < p.w.rows) {
 #pragma unroll
@@ -491,7 +455,14 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     if (warp == S::kIssue) tmem_free<S::PAIR>(tmem, S::kTmem);
     if (threadIdx.x == 0 && *gave_up) set_flag(flags, VF_FLAG_GAVE_UP);
     __syncwarp();
-    if (in_cluster) cluster_sync();  // no CTA ends while another one reads its sums
+    // no CTA ends while another one may still write to it
+    if (S::PAIR) {
+        cluster_sync();
+    } else {
+        if (!joined) cluster_wait();
+        if (!left) cluster_arrive_relaxed();
+        if (in_cluster) cluster_wait();
+    }
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -538,42 +509,64 @@ void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
     const int64_t n_tiles = (p.w.rows + S::kOutputs - 1) / S::kOutputs;
     const int64_t tiles = most_row_tiles(p, S::kTokens) * n_tiles;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned(std::min<int64_t>(tiles, std::max(1, ctx->sm_count * S::PER_SM / ranks)) * ranks));
+    cfg.gridDim = dim3(unsigned((S::SWAP && ranks > 1 ? tiles : std::min<int64_t>(tiles, ctx->sm_count * S::PER_SM / ranks)) * ranks));
     cfg.blockDim = dim3(S::kThreads);
     cfg.dynamicSmemBytes = S::kSmem;
     cfg.stream = ctx->stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = unsigned(ranks);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (see chain_enter)
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(ranks);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
     const uint32_t idesc = tc_f8_shape((S::SWAP ? p.w : p.x).dtype == VF_DT_F8E5M2, (S::SWAP ? p.x : p.w).dtype == VF_DT_F8E5M2, S::PAIR ? 256 : 128, S::BN);
     VF_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_codes(p.x, 2, S::PAIR ? 128 : S::kTokens), map_codes(p.w, 3, S::SWAP ? 128 : S::kRowsB), p, int(n_tiles), idesc, ctx->d_flags));
 }
 
 //                       BN, stages, accumulators, epilogue groups of four warps, CTAs per SM
-using Swap16 = Shape<Form::kSwap, 16, 5, 4, 1, 2>;
-using Swap32 = Shape<Form::kSwap, 32, 4, 4, 1, 2>;
-using Swap64 = Shape<Form::kSwap, 64, 4, 4, 1, 2>;
+using Swap16 = Shape<Form::kSwap, 16, 5, 4, 1, 2, 16>;
+using Swap32 = Shape<Form::kSwap, 32, 4, 4, 1, 2, 16>;
+using Swap64 = Shape<Form::kSwap, 64, 3, 4, 1, 2, 16>;
 using Single64 = Shape<Form::kSingle, 64, 3, 4, 1, 2>;
 using Single128 = Shape<Form::kSingle, 128, 5, 2, 2, 1>;
 using Pair256 = Shape<Form::kPair, 256, 5, 2, 2, 1, 16>;
+
+// CTAs that share a tile's column blocks: the number with which the busiest multiprocessor has the fewest column blocks to
+// read, at two CTAs per multiprocessor, where every tile has a cluster of its own. Joining costs about as much as four blocks.
+template <class S>
+int ranks_for(vf_ctx* ctx, int64_t tiles, int64_t col_blocks) {
+    int best = 1;
+    int64_t least = INT64_MAX;
+    for (int r = 1; r <= 8 && (r == 1 || (tiles * r <= 2 * ctx->sm_count && 2 * r <= col_blocks)); ++r) {
+        if (r > 1 && (S::kFours + r - 1) / r * r > S::kParts) continue;
+        const int64_t ctas = std::min<int64_t>(tiles * r, 2 * ctx->sm_count), rounds = (tiles * r + ctas - 1) / ctas;
+        const int64_t load = rounds * ((ctas + ctx->sm_count - 1) / ctx->sm_count) * ((col_blocks + r - 1) / r + (r > 1 ? 4 : 0));
+        if (load < least) {
+            least = load;
+            best = r;
+        }
+    }
+    return best;
+}
+
+template <class S, class T>
+void launch_swapped(vf_ctx* ctx, const BlockProduct& p) {
+    launch_tensor<S, T>(ctx, p, ranks_for<S>(ctx, most_row_tiles(p, S::BN) * ((p.w.rows + 127) / 128), p.x.col_blocks));
+}
 
 template <class T>
 void launch_for(vf_ctx* ctx, const BlockProduct& p) {
     if (!fits_bulk_copies(p.x) || !fits_bulk_copies(p.w)) return launch_plain<T>(ctx, p);
     const int64_t rows = p.offsets ? (p.x.rows + p.w.count - 1) / p.w.count : p.x.rows;
     const int64_t n_tiles = (p.w.rows + 127) / 128;
-    if (rows <= 32) {
-        const int bn = rows <= 16 ? 16 : 32;
-        const int64_t tiles = most_row_tiles(p, bn) * n_tiles;
-        int ranks = 1;
-        while (ranks < 8 && tiles * ranks * 2 <= 2 * ctx->sm_count && p.x.col_blocks >= 4 * ranks) ranks *= 2;
-        if (bn == 16) launch_tensor<Swap16, T>(ctx, p, ranks);
-        else launch_tensor<Swap32, T>(ctx, p, ranks);
+    if (rows <= 16) {
+        launch_swapped<Swap16, T>(ctx, p);
+    } else if (rows <= 32) {
+        launch_swapped<Swap32, T>(ctx, p);
     } else if (rows <= 64) {
-        launch_tensor<Swap64, T>(ctx, p);
+        launch_swapped<Swap64, T>(ctx, p);
     } else {
         if (most_row_tiles(p, 256) * ((p.w.rows + 255) / 256) >= ctx->sm_count / 2) launch_tensor<Pair256, T>(ctx, p);
         else if (most_row_tiles(p, 128) * n_tiles >= ctx->sm_count) launch_tensor<Single128, T>(ctx, p);

@@ -118,6 +118,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int n) {
 template <class T, bool E5M2, bool Aligned>
 __global__ void __launch_bounds__(kThreads) k_quantize_tokens(const T* __restrict__ base, int64_t base_ld, Blocks b, int64_t col_tiles,
                                                               int64_t tiles, int* flags) {
+    chain_enter();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l16 = lane & 15;
     const int64_t all_rows = b.count * b.rows;
     for (int64_t t = blockIdx.x; t < tiles; t += gridDim.x) {
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(kThreads) k_quantize_tokens(const T* __restric
 // maximum is taken; the elements stay in registers until the codes are written.
 template <class T, bool E5M2, bool Aligned>
 __global__ void __launch_bounds__(kThreads) k_quantize_weights(const T* __restrict__ base, int64_t base_ld, Blocks b, int64_t tiles, int* flags) {
+    chain_enter();
     constexpr int kIter = kBlock / (kThreads / 16);
     __shared__ uint32_t tops[2][kThreads / 32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(kThreads) k_quantize_weights(const T* __restri
 // every store instruction of a warp is one run of 512 bytes; four rows are in flight per warp.
 template <class T, bool E5M2, bool Aligned>
 __global__ void __launch_bounds__(kThreads) k_dequantize_blocks(Blocks b, T* __restrict__ dst, int64_t dst_ld, int64_t col_tiles, int64_t tiles) {
+    chain_enter();
     constexpr int kPer = 16 / sizeof(T);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t all_rows = b.count * b.rows;
@@ -295,10 +298,10 @@ void launch_quantize_blocks(vf_ctx* ctx, const void* base, int base_dt, int64_t 
                 const T* src = static_cast<const T*>(base);
                 if (b.block_rows == 1) {
                     const int64_t ct = (b.col_blocks + 1) / 2, tiles = ct * ((b.count * b.rows + kTileRows - 1) / kTileRows);
-                    k_quantize_tokens<T, e5.value, vec.value><<<grid_for(tiles), kThreads, 0, ctx->stream>>>(src, base_ld, b, ct, tiles, ctx->d_flags);
+                    VF_CUDA(launch_chained(k_quantize_tokens<T, e5.value, vec.value>, dim3(grid_for(tiles)), dim3(kThreads), 0, ctx->stream, src, base_ld, b, ct, tiles, ctx->d_flags));
                 } else {
                     const int64_t tiles = b.count * b.row_blocks * b.col_blocks;
-                    k_quantize_weights<T, e5.value, vec.value><<<grid_for(tiles), kThreads, 0, ctx->stream>>>(src, base_ld, b, tiles, ctx->d_flags);
+                    VF_CUDA(launch_chained(k_quantize_weights<T, e5.value, vec.value>, dim3(grid_for(tiles)), dim3(kThreads), 0, ctx->stream, src, base_ld, b, tiles, ctx->d_flags));
                 }
             });
         });
@@ -314,7 +317,7 @@ void launch_dequantize_blocks(vf_ctx* ctx, const Blocks& b, void* dst, int dst_d
         with_flag(b.dtype == VF_DT_F8E5M2, [&](auto e5) {
             with_flag(al, [&](auto vec) {
                 using T = decltype(t);
-                k_dequantize_blocks<T, e5.value, vec.value><<<grid_for(tiles), kThreads, 0, ctx->stream>>>(b, static_cast<T*>(dst), dst_ld, ct, tiles);
+                VF_CUDA(launch_chained(k_dequantize_blocks<T, e5.value, vec.value>, dim3(grid_for(tiles)), dim3(kThreads), 0, ctx->stream, b, static_cast<T*>(dst), dst_ld, ct, tiles));
             });
         });
     });

@@ -34,13 +34,6 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// arrives at the barrier that lies at the same address in CTA `rank` of the cluster; releases to the whole cluster
-__device__ __forceinline__ void bar_arrive_at(uint32_t bar, uint32_t rank) {
-    asm volatile(
-        "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tmbarrier.arrive.release.cluster.shared::cluster.b64 _, [a];\n\t}" ::"r"(bar),
-        "r"(rank)
-        : "memory");
-}
 __device__ __forceinline__ uint32_t bar_at_rank(uint32_t bar, uint32_t rank) {  // the same barrier of another CTA of the cluster
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(bar), "r"(rank));
@@ -51,19 +44,12 @@ __device__ __forceinline__ uint32_t bar_at_rank(uint32_t bar, uint32_t rank) {  
 __device__ __forceinline__ void bar_arrive_remote(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-template <bool Cluster>
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
-    if constexpr (Cluster)
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok)
-                     : "r"(bar), "r"(parity)
-                     : "memory");
-    else
-        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-                     : "=r"(ok)
-                     : "r"(bar), "r"(parity)
-                     : "memory");
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok)
+                 : "r"(bar), "r"(parity)
+                 : "memory");
     return ok != 0;
 }
 __device__ __forceinline__ uint64_t global_ns() {
@@ -77,12 +63,11 @@ constexpr uint64_t kDrainLimitNs = 1000000;    // and after one gave up, copies 
 
 // Waits until the phase `parity` of the barrier is complete. Gives up after the time limit, or when another thread of the
 // CTA has: `gave_up` (shared memory) is then set and false is returned.
-template <bool Cluster = false>
 __device__ __forceinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, volatile int* gave_up) {
     const uint64_t t0 = global_ns();
     for (;;) {
         for (int i = 0; i < 64; ++i)
-            if (bar_try<Cluster>(bar, parity)) return true;
+            if (bar_try(bar, parity)) return true;
         if (*gave_up) return false;
         if (global_ns() - t0 > kWaitLimitNs) {
             *gave_up = 1;
@@ -90,11 +75,10 @@ __device__ __forceinline__ bool bar_wait_long(uint32_t bar, uint32_t parity, vol
         }
     }
 }
-template <bool Cluster = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
     for (int i = 0; i < 1024; ++i)  // (reading the clock would delay a wait that is about to end)
-        if (bar_try<Cluster>(bar, parity)) return true;
-    return bar_wait_long<Cluster>(bar, parity, gave_up);
+        if (bar_try(bar, parity)) return true;
+    return bar_wait_long(bar, parity, gave_up);
 }
 
 // ---- clusters --------------------------------------------------------------------------------------------------------
@@ -111,10 +95,22 @@ __device__ __forceinline__ uint32_t cluster_size() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float load_from_rank(uint32_t addr, uint32_t rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
-    return v;
+__device__ __forceinline__ void cluster_arrive() {  // its wait orders the barriers that were initialised before
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_arrive_relaxed() {
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+    asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+// Four words to shared memory of CTA `rank` of the cluster, counted off from what its barrier `bar` expects. Needs no fence.
+__device__ __forceinline__ void push_to_rank(uint32_t dst, uint32_t bar, uint32_t rank, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile(
+        "{\n\t.reg .b32 p, q;\n\tmapa.shared::cluster.u32 p, %0, %2;\n\tmapa.shared::cluster.u32 q, %1, %2;\n\t"
+        "st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [p], {%3, %4, %5, %6}, [q];\n\t}" ::"r"(dst),
+        "r"(bar), "r"(rank), "r"(a), "r"(b), "r"(c), "r"(d)
+        : "memory");
 }
 
 // ---- asynchronous copies of single words -------------------------------------------------------------------------------
@@ -245,6 +241,11 @@ __device__ __forceinline__ void tmem_load_wait(uint32_t (&v)[32]) {
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) {
     uint64_t r;
     asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
 __device__ __forceinline__ void fma2(uint64_t& acc, uint64_t a, uint64_t b) {
