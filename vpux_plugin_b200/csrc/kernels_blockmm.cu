@@ -1,6 +1,8 @@
 // Products of matrices of 8-bit floats with a scale per block of 128 columns, plain or grouped by expert.
 //
 //   y[m][n] = sum over column blocks b of  (sx[m][b] * sw[n / 128][b]) * sum over k in b of cx[m][k] * cw[n][k]
+#include <atomic>
+
 #include "block_device.cuh"
 #include "tensor_core.cuh"
 
@@ -114,7 +116,7 @@ struct Shape {
     static constexpr int kStageBytes = (128 + kRowsB) * kBlock;
     static constexpr int kTmem = NBUF * BN < 32 ? 32 : NBUF * BN;
     // clusters share a tile's column blocks: four columns of a tile at a time, the CTAs of a cluster own them in turn
-    static constexpr int kFours = BN / 4, kParts = BN == 16 ? 8 : (BN == 32 ? 10 : 16);
+    static constexpr int kFours = BN / 4, kParts = BN == 16 ? 8 : (BN == 32 ? 10 : BN / 4);
     static constexpr int kRing = STAGES * kStageBytes;
     static constexpr int kScales = kSlots * kSlotBytes;
     static constexpr int kExtra = SWAP ? kParts * 128 * 16 : 4 * GROUPS * 4096;  // partial sums; results on their way out
@@ -150,10 +152,11 @@ __device__ __forceinline__ void store_rows(char* stage, T* out, int64_t ld, cons
                 if (r < rows) *reinterpret_cast<uint4*>(out + r * ld + c + u * kPer) = v;
             }
         } else {
-            for (int r = 0; r < rows; ++r)
+#pragma unroll 8
+            for (int r = 0; r < 32; ++r)
 #pragma unroll
                 for (int k = lane; k < kChunk; k += 32)
-                    if (c + k < cols) out[r * ld + c + k] = *reinterpret_cast<const T*>(stage + r * 128 + ((k / kPer ^ r) & 7) * 16 + k % kPer * sizeof(T));
+                    if (r < rows && c + k < cols) out[r * ld + c + k] = *reinterpret_cast<const T*>(stage + r * 128 + ((k / kPer ^ r) & 7) * 16 + k % kPer * sizeof(T));
         }
     }
 }
@@ -214,9 +217,17 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     bool joined = !in_cluster, left = !in_cluster;
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
-    chain_enter();  // set up while the kernel before this one was ending; from here on its results are read
-
     const int kbs = int(p.x.col_blocks), kb0 = int(rank * uint32_t(kbs) / ranks), kb1 = int((rank + 1) * uint32_t(kbs) / ranks);
+    // Set up while the kernel before this one was ending; from chain_enter() on its results are read. The weights of the first
+    // tile are asked for before that: into the L2 cache, where it does not matter whether that kernel writes them.
+    if (warp == S::kCopies && !p.offsets) {
+        const int64_t t = blockIdx.x / (S::PAIR ? 2 : ranks);
+        const int n_tile = int(t / ((p.x.rows + S::kTokens - 1) / S::kTokens));
+        if (lane < STAGES && kb0 + lane < kb1 && n_tile < n_tiles) tma_prefetch_3d(&wmap, (kb0 + lane) * kBlock, n_tile * S::kOutputs + int(half) * S::kRowsB, 0);
+        __syncwarp();
+    }
+    chain_enter();
+
     // The next tile, as the copying warp has found it; by whole warps
     int4 tile;
     uint32_t turn = 0;
@@ -412,10 +423,12 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                     joined = true;
                     const uint32_t my_place = smem_addr(extra) + (rank * places * 128 + quarter * 32 + lane) * 16;
 #pragma unroll
-                    for (int g = 0; g < S::kFours; ++g)
+                    for (int i = 0; i < kCols / 4; ++i) {
+                        const int g = col0 / 4 + i;
                         if (g < fours)
-                            push_to_rank(my_place + g / int(ranks) * 128 * 16, parts_full, g % int(ranks), uint32_t(acc[2 * g]), uint32_t(acc[2 * g] >> 32),
-                                         uint32_t(acc[2 * g + 1]), uint32_t(acc[2 * g + 1] >> 32));
+                            push_to_rank(my_place + g / int(ranks) * 128 * 16, parts_full, g % int(ranks), uint32_t(acc[2 * i]), uint32_t(acc[2 * i] >> 32),
+                                         uint32_t(acc[2 * i + 1]), uint32_t(acc[2 * i + 1] >> 32));
+                    }
                     __syncwarp();
                     cluster_arrive_relaxed();
                     left = true;
@@ -423,7 +436,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                     ok = __all_sync(0xffffffffu, bar_wait(parts_full, 0, gave_up));
                     if (!ok) break;
                     const float4* const parts = reinterpret_cast<const float4*>(extra) + quarter * 32 + lane;
-                    for (int j = 0; j < mine; ++j) {
+                    for (int j = warp / 4; j < mine; j += S::GROUPS) {
                         float4 v = parts[j * 128];
                         for (int r = 1; r < int(ranks); ++r) {
                             const float4 q = parts[(r * places + j) * 128];
@@ -485,8 +498,15 @@ CUtensorMap map_codes(const Blocks& b, int rank, int box_rows) {
     const cuuint64_t dim[3] = {cuuint64_t(b.cols), cuuint64_t(b.rows), cuuint64_t(b.count)};
     const cuuint64_t stride[2] = {cuuint64_t(b.ld), cuuint64_t(b.count > 1 ? b.matrix_stride : b.ld)};
     const cuuint32_t box[3] = {kBlock, cuuint32_t(box_rows), 1}, one[3] = {1, 1, 1};
-    const CUresult r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank), b.codes, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    CUresult r = CUDA_SUCCESS;
+    for (int attempt = 0; attempt < 2; ++attempt) {
+        r = encode_tiled()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank), b.codes, dim, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+        if (r != CUDA_ERROR_INVALID_CONTEXT) break;
+        int dev = 0;  // a thread's first call of the driver: let the runtime make its context current
+        VF_CUDA(cudaGetDevice(&dev));
+        VF_CUDA(cudaSetDevice(dev));
+    }
     if (r != CUDA_SUCCESS) raise(VF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
     return m;
 }
@@ -500,11 +520,16 @@ template <class S, class T>
 void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
     if (S::PAIR) ranks = 2;
     auto kernel = k_matmul_blocks<S, T>;
-    VF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
-    if (S::kTrades) {  // warps that take registers wait until they are there: what is taken has to have been given
-        cudaFuncAttributes fa;
-        VF_CUDA(cudaFuncGetAttributes(&fa, kernel));
-        if (fa.numRegs * S::kThreads < 128 * kGiven + 128 * S::GROUPS * kTaken) raise(VF_ERR_CUDA, "the kernel was built with too few registers");
+    static std::atomic<uint64_t> ready{0};  // devices (below 64) on which this kernel has been set up
+    const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
+    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+        VF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        if (S::kTrades) {  // warps that take registers wait until they are there: what is taken has to have been given
+            cudaFuncAttributes fa;
+            VF_CUDA(cudaFuncGetAttributes(&fa, kernel));
+            if (fa.numRegs * S::kThreads < 128 * kGiven + 128 * S::GROUPS * kTaken) raise(VF_ERR_CUDA, "the kernel was built with too few registers");
+        }
+        ready.fetch_or(bit, std::memory_order_relaxed);
     }
     const int64_t n_tiles = (p.w.rows + S::kOutputs - 1) / S::kOutputs;
     const int64_t tiles = most_row_tiles(p, S::kTokens) * n_tiles;
@@ -529,21 +554,21 @@ void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
 using Swap16 = Shape<Form::kSwap, 16, 5, 4, 1, 2, 16>;
 using Swap32 = Shape<Form::kSwap, 32, 4, 4, 1, 2, 16>;
 using Swap64 = Shape<Form::kSwap, 64, 3, 4, 1, 2, 16>;
+using Swap128 = Shape<Form::kSwap, 128, 4, 2, 2, 1, 16>;
 using Single64 = Shape<Form::kSingle, 64, 3, 4, 1, 2>;
 using Single128 = Shape<Form::kSingle, 128, 5, 2, 2, 1>;
 using Pair256 = Shape<Form::kPair, 256, 5, 2, 2, 1, 16>;
 
-// CTAs that share a tile's column blocks: the number with which the busiest multiprocessor has the fewest column blocks to
-// read, at two CTAs per multiprocessor, where every tile has a cluster of its own. Joining costs about as much as four blocks.
+// CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column blocks
+// that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs about as much as
+// four of them. (48 rows, 4096 x 11008, 32 tiles of 86 blocks: 18.7 us with four, 13.5 with eight.)
 template <class S>
 int ranks_for(vf_ctx* ctx, int64_t tiles, int64_t col_blocks) {
     int best = 1;
-    int64_t least = INT64_MAX;
-    for (int r = 1; r <= 8 && (r == 1 || (tiles * r <= 2 * ctx->sm_count && 2 * r <= col_blocks)); ++r) {
-        if (r > 1 && (S::kFours + r - 1) / r * r > S::kParts) continue;
-        const int64_t ctas = std::min<int64_t>(tiles * r, 2 * ctx->sm_count), rounds = (tiles * r + ctas - 1) / ctas;
-        const int64_t load = rounds * ((ctas + ctx->sm_count - 1) / ctx->sm_count) * ((col_blocks + r - 1) / r + (r > 1 ? 4 : 0));
-        if (load < least) {
+    int64_t least = col_blocks;
+    for (int r = 2; r <= 8 && tiles * r <= S::PER_SM * ctx->sm_count && 2 * r <= col_blocks; ++r) {
+        const int64_t load = (col_blocks + r - 1) / r + 4;
+        if ((S::kFours + r - 1) / r * r <= S::kParts && load < least) {
             least = load;
             best = r;
         }
@@ -567,6 +592,8 @@ void launch_for(vf_ctx* ctx, const BlockProduct& p) {
         launch_swapped<Swap32, T>(ctx, p);
     } else if (rows <= 64) {
         launch_swapped<Swap64, T>(ctx, p);
+    } else if (most_row_tiles(p, 128) * n_tiles * 2 <= ctx->sm_count) {
+        launch_swapped<Swap128, T>(ctx, p);
     } else {
         if (most_row_tiles(p, 256) * ((p.w.rows + 255) / 256) >= ctx->sm_count / 2) launch_tensor<Pair256, T>(ctx, p);
         else if (most_row_tiles(p, 128) * n_tiles >= ctx->sm_count) launch_tensor<Single128, T>(ctx, p);

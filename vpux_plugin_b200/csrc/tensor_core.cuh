@@ -154,6 +154,10 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, 
                      : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* m, int x, int y, int z) {  // into the L2 cache
+    asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(m), "r"(x), "r"(y), "r"(z) : "memory");
+}
+
 // ---- tensor core -------------------------------------------------------------------------------------------------------
 // Pair: the two CTAs of a pair (cluster ranks 2i and 2i + 1) work on one tile. Both allocate and free, the even one issues.
 template <bool Pair>

@@ -16,6 +16,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libvfold.so")
 
 
+_Err = C.c_char * 512
+
+
 class VfoldError(RuntimeError):
     def __init__(self, status, msg):
         super().__init__(f"[{status}] {msg}")
@@ -160,7 +163,7 @@ class Library:
     # -- plumbing -------------------------------------------------------------------------------------
     @staticmethod
     def _err():
-        return C.create_string_buffer(512)
+        return _Err()
 
     @staticmethod
     def _check(st, err):
