@@ -73,9 +73,7 @@ struct TileWalk {
     __device__ __forceinline__ void load() {
         const int e = e0 + int(threadIdx.x & 31);
         lo = hi = 0;
-        if (!offsets) {
-            if (e == 0) hi = int(rows);
-        } else if (e < experts) {
+        if (e < experts) {
             const int64_t a = offsets[e], b = offsets[e + 1];
             const int64_t ca = a < 0 ? 0 : (a > rows ? rows : a), cb = b < ca ? ca : (b > rows ? rows : b);
             if (a != ca || b != cb) set_flag(flags, VF_FLAG_OFFSETS);
@@ -98,10 +96,19 @@ struct TileWalk {
         flags = err_flags;
         e0 = 0;
         base = 0;
-        load();
+        if (offsets) load();
     }
     // Finds tile `t` (not below the one found before); false behind the last tile.
     __device__ __forceinline__ bool find(int64_t t) {
+        if (!offsets) {  // one group: nothing to search
+            const int m_tiles = (int(rows) + bm - 1) / bm;
+            if (t >= int64_t(m_tiles) * n_tiles) return false;
+            n_tile = int(uint32_t(t) / uint32_t(m_tiles));
+            expert = 0;
+            row0 = (int(t) - n_tile * m_tiles) * bm;
+            row_end = int(rows);
+            return true;
+        }
         for (;;) {
             const int64_t here = __shfl_sync(0xffffffffu, through, 31);
             if (t - base < here) break;

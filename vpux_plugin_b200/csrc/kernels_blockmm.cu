@@ -437,13 +437,16 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                     if (!ok) break;
                     const float4* const parts = reinterpret_cast<const float4*>(extra) + quarter * 32 + lane;
                     for (int j = warp / 4; j < mine; j += S::GROUPS) {
-                        float4 v = parts[j * 128];
-                        for (int r = 1; r < int(ranks); ++r) {
-                            const float4 q = parts[(r * places + j) * 128];
-                            v.x = __fadd_rn(v.x, q.x);
-                            v.y = __fadd_rn(v.y, q.y);
-                            v.z = __fadd_rn(v.z, q.z);
-                            v.w = __fadd_rn(v.w, q.w);
+                        float4 q[8];  // all of them on their way before the first is added
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) q[r] = r < int(ranks) ? parts[(r * places + j) * 128] : make_float4(0.f, 0.f, 0.f, 0.f);
+                        float4 v = q[0];
+#pragma unroll
+                        for (int r = 1; r < 8; ++r) {
+                            v.x = __fadd_rn(v.x, q[r].x);
+                            v.y = __fadd_rn(v.y, q[r].y);
+                            v.z = __fadd_rn(v.z, q[r].z);
+                            v.w = __fadd_rn(v.w, q[r].w);
                         }
                         const int i = 4 * (int(rank) + j * int(ranks));
                         if (n >= p.w.rows) continue;
