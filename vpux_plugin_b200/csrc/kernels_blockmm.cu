@@ -94,27 +94,20 @@ void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
 // the ranks.
 constexpr int kGiven = 72, kTaken = 216;  // registers per thread after the trade: 128 * 72 + 256 * 216 = 384 * 168
 
-enum class Form {
-    kSwap,    // the weights are the 128-row operand, BN activations the other one
-    kSingle,  // 128 activations are the 128-row operand, BN outputs the other one
-    kPair     // the same with 256 activations on a pair of CTAs, which share the BN outputs' weights
-};
-
-template <Form FORM_, int BN_, int STAGES_, int NBUF_, int GROUPS_, int PER_SM_, int LOAD_ = 32>
+template <bool SWAP_, int BN_, int STAGES_, int NBUF_, int GROUPS_, int PER_SM_, int LOAD_ = 32>
 struct Shape {
-    static constexpr bool SWAP = FORM_ == Form::kSwap, PAIR = FORM_ == Form::kPair;
+    static constexpr bool SWAP = SWAP_;  // the weights are the 128-row operand; else the activations are
     static constexpr int BN = BN_, STAGES = STAGES_, NBUF = NBUF_, GROUPS = GROUPS_, PER_SM = PER_SM_, LOAD = LOAD_;
     static constexpr int kCols = BN / GROUPS;               // columns of the accumulator per epilogue warp
-    static constexpr int kTokens = SWAP ? BN : (PAIR ? 256 : 128), kOutputs = SWAP ? 128 : BN;  // a tile's results
+    static constexpr int kTokens = SWAP ? BN : 128, kOutputs = SWAP ? 128 : BN;  // a tile's results
     static constexpr int kEpilogue = 4 * GROUPS, kCopies = kEpilogue, kIssue = kEpilogue + 1, kScaling = kEpilogue + 2;  // warps
     static constexpr bool kTrades = kCols > 64;             // the warps behind the epilogue's give it registers, as a group of four
     static constexpr int kThreads = 32 * (kEpilogue + (kTrades ? 4 : 3));
-    // scales of kAhead column blocks at a time: [kAhead][kTileRows] of the activations, [kTileBlocks][kAhead] of the weights
-    static constexpr int kAhead = 8, kSlots = 2, kTileRows = SWAP ? BN : 128, kTileBlocks = SWAP ? 1 : 2;
+    // scales of kAhead column blocks at a time: [kAhead][kTileRows] of the activations, [kTileBlocks][kAhead] of the weights of an epilogue group's columns
+    static constexpr int kAhead = 8, kSlots = 2, kTileRows = SWAP ? BN : 128, kTileBlocks = SWAP ? 1 : GROUPS;
     static constexpr int kSlotBytes = kAhead * (kTileRows + kTileBlocks) * 4;
-    static constexpr int kRowsB = PAIR ? BN / 2 : BN;       // rows of the second operand that this CTA holds
-    static constexpr int kStageBytes = (128 + kRowsB) * kBlock;
-    static constexpr int kTmem = NBUF * BN < 32 ? 32 : NBUF * BN;
+    static constexpr int kStageBytes = (128 + BN) * kBlock;
+    static constexpr int kTmem = NBUF * BN <= 64 ? 64 : (NBUF * BN <= 128 ? 128 : (NBUF * BN <= 256 ? 256 : 512));  // a power of two
     // clusters share a tile's column blocks: four columns of a tile at a time, the CTAs of a cluster own them in turn
     static constexpr int kFours = BN / 4, kParts = BN == 16 ? 8 : (BN == 32 ? 10 : BN / 4);
     static constexpr int kRing = STAGES * kStageBytes;
@@ -161,6 +154,18 @@ __device__ __forceinline__ void store_rows(char* stage, T* out, int64_t ld, cons
     }
 }
 
+// Position in a ring of N and the phase of its barriers; the producer of a ring waits for the other phase than its consumer.
+template <int N>
+struct RingAt {
+    uint32_t i = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++i == N) {
+            i = 0;
+            phase ^= 1;
+        }
+    }
+};
+
 template <class S, class T>
 __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     k_matmul_blocks(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, const __grid_constant__ BlockProduct p, int n_tiles,
@@ -183,8 +188,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ranks = S::SWAP ? cluster_size() : 1, rank = S::SWAP ? cluster_rank() : 0;  // CTAs that share a tile's column blocks
-    const uint32_t half = S::PAIR ? cluster_rank() : 0;
-    const bool in_cluster = S::PAIR || ranks > 1;
+    const bool in_cluster = ranks > 1;
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             bar_init(full + 8 * i, 1);
@@ -192,7 +196,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         }
         for (int i = 0; i < NBUF; ++i) {
             bar_init(done + 8 * i, 1);
-            bar_init(taken + 8 * i, (S::PAIR ? 8 : 4) * S::GROUPS);
+            bar_init(taken + 8 * i, 4 * S::GROUPS);
         }
         bar_init(parts_full, 1);
         bar_init(drained, 1);
@@ -209,11 +213,10 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         tma_prefetch_map(&xmap);
         tma_prefetch_map(&wmap);
     }
-    if (warp == S::kIssue) tmem_alloc<S::PAIR>(smem_addr(tmem_at), S::kTmem);
+    if (warp == S::kIssue) tmem_alloc(smem_addr(tmem_at), S::kTmem);
     tc_fence_before();
     __syncthreads();
-    if (S::PAIR) cluster_sync();
-    else if (in_cluster) cluster_arrive();  // waited for before anything goes to another CTA
+    if (in_cluster) cluster_arrive();  // waited for before anything goes to another CTA
     bool joined = !in_cluster, left = !in_cluster;
     tc_fence_after();
     const uint32_t tmem = *tmem_at;
@@ -221,9 +224,9 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     // Set up while the kernel before this one was ending; from chain_enter() on its results are read. The weights of the first
     // tile are asked for before that: into the L2 cache, where it does not matter whether that kernel writes them.
     if (warp == S::kCopies && !p.offsets) {
-        const int64_t t = blockIdx.x / (S::PAIR ? 2 : ranks);
+        const int64_t t = blockIdx.x / ranks;
         const int n_tile = int(t / ((p.x.rows + S::kTokens - 1) / S::kTokens));
-        if (lane < STAGES && kb0 + lane < kb1 && n_tile < n_tiles) tma_prefetch_3d(&wmap, (kb0 + lane) * kBlock, n_tile * S::kOutputs + int(half) * S::kRowsB, 0);
+        if (lane < STAGES && kb0 + lane < kb1 && n_tile < n_tiles) tma_prefetch_3d(&wmap, (kb0 + lane) * kBlock, n_tile * S::kOutputs, 0);
         __syncwarp();
     }
     chain_enter();
@@ -244,12 +247,12 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     if (warp >= S::kEpilogue) {
     if constexpr (S::kTrades) regs_give<kGiven>();
     if (warp == S::kCopies) {  // ---- finding tiles, copying them in
-        const uint32_t sharing = S::PAIR ? 2 : ranks;
         TileWalk walk;
         walk.start(p.offsets, p.offsets ? int(p.w.count) : 1, p.x.rows, S::kTokens, n_tiles, flags);
         uint32_t it = 0;
+        RingAt<STAGES> at_stage;
         bool ok = true;
-        for (int64_t t = blockIdx.x / sharing; ok; t += gridDim.x / sharing, ++turn) {
+        for (int64_t t = blockIdx.x / ranks; ok; t += gridDim.x / ranks, ++turn) {
             const bool more = walk.find(t);
             const uint32_t i = turn & 1;
             ok = __all_sync(0xffffffffu, bar_wait(tile_read + 8 * i, ((turn >> 1) & 1) ^ 1, gave_up));
@@ -259,15 +262,14 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                 bar_arrive(tile_there + 8 * i);
             }
             if (!more) break;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t s = it % STAGES, at = smem_addr(ring) + s * S::kStageBytes;
-                const uint32_t bar = S::PAIR ? bar_at_rank(full + 8 * s, 0) : full + 8 * s;
-                ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, ((it / STAGES) & 1) ^ 1, gave_up));
+            for (int kb = kb0; kb < kb1; ++kb, ++it, at_stage.next()) {
+                const uint32_t s = at_stage.i, at = smem_addr(ring) + s * S::kStageBytes;
+                ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, at_stage.phase ^ 1, gave_up));
                 if (!ok) break;
                 if (elect_one()) {
-                    if (half == 0) bar_expect(full + 8 * s, S::PAIR ? 2 * S::kStageBytes : S::kStageBytes);
-                    tma_load_3d<S::PAIR>(S::SWAP ? at : at + 128 * kBlock, &wmap, bar, kb * kBlock, walk.n_tile * S::kOutputs + int(half) * S::kRowsB, walk.expert);
-                    tma_load_2d<S::PAIR>(S::SWAP ? at + 128 * kBlock : at, &xmap, bar, kb * kBlock, walk.row0 + int(half) * 128);
+                    bar_expect(full + 8 * s, S::kStageBytes);
+                    tma_load_3d(S::SWAP ? at : at + 128 * kBlock, &wmap, full + 8 * s, kb * kBlock, walk.n_tile * S::kOutputs, walk.expert);
+                    tma_load_2d(S::SWAP ? at + 128 * kBlock : at, &xmap, full + 8 * s, kb * kBlock, walk.row0);
                 }
             }
         }
@@ -276,45 +278,45 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         if (!ok && lane == 0)  // the copies in flight land before the CTA ends
             for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
                 const uint64_t t0 = global_ns();
-                while (!(half == 0 && bar_try(full + 8 * (i % STAGES), (i / STAGES) & 1)) && global_ns() - t0 < kDrainLimitNs) {
+                while (!bar_try(full + 8 * (i % STAGES), (i / STAGES) & 1) && global_ns() - t0 < kDrainLimitNs) {
                 }
             }
     } else if (warp == S::kIssue) {  // ---- matrix instructions
-        uint32_t it = 0;
+        RingAt<STAGES> at_stage;
+        RingAt<NBUF> at_sum;
         bool ok = true;
         while (ok && next_tile()) {
-            if (half != 0) continue;
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const uint32_t s = it % STAGES, b = it % NBUF;
-                ok = __all_sync(0xffffffffu, bar_wait(taken + 8 * b, ((it / NBUF) & 1) ^ 1, gave_up) && bar_wait(full + 8 * s, (it / STAGES) & 1, gave_up));
-                if (!ok) break;
-                tc_fence_after();
+            for (int kb = kb0; kb < kb1; ++kb, at_stage.next(), at_sum.next()) {
+                const uint32_t s = at_stage.i, b = at_sum.i;
                 const uint32_t at = smem_addr(ring) + s * S::kStageBytes;
                 const uint64_t ad = tc_operand(at), bd = tc_operand(at + 128 * kBlock);
+                // the accumulator last: with it the time between two uses of one accumulator starts to run
+                ok = __all_sync(0xffffffffu, bar_wait(full + 8 * s, at_stage.phase, gave_up) && bar_wait(taken + 8 * b, at_sum.phase ^ 1, gave_up));
+                if (!ok) break;
+                tc_fence_after();
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8<S::PAIR>(tmem + b * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0);
-                    tc_commit<S::PAIR>(empty + 8 * s);
-                    tc_commit<S::PAIR>(done + 8 * b);
+                    for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8(tmem + b * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0);
+                    tc_commit(done + 8 * b);
+                    tc_commit(empty + 8 * s);
                 }
             }
         }
         if (!ok && elect_one()) {  // the instructions in flight end before their memory is given back
-            tc_commit<S::PAIR>(drained);
+            tc_commit(drained);
             const uint64_t t0 = global_ns();
             while (!bar_try(drained, 0) && global_ns() - t0 < kDrainLimitNs) {
             }
         }
     } else if (warp == S::kScaling) {  // ---- scales of kAhead column blocks into the next slot, by asynchronous copies
-        uint32_t chunk = 0;
+        RingAt<S::kSlots> at_slot;
         bool ok = true;
         while (ok && next_tile()) {
-            const int row = tile.y + int(half) * 128 + lane;
+            const int row = tile.y + lane;
             const float* const sx = p.x.scales + row * p.x.srs;
-            const int64_t wb0 = int64_t(tile.w) * S::kOutputs / 128;
-            for (int kb = kb0; kb < kb1; kb += S::kAhead, ++chunk) {
-                const uint32_t slot = chunk % S::kSlots, at = smem_addr(scales) + slot * S::kSlotBytes;
-                ok = __all_sync(0xffffffffu, bar_wait(slot_read + 8 * slot, ((chunk / S::kSlots) & 1) ^ 1, gave_up));
+            for (int kb = kb0; kb < kb1; kb += S::kAhead, at_slot.next()) {
+                const uint32_t slot = at_slot.i, at = smem_addr(scales) + slot * S::kSlotBytes;
+                ok = __all_sync(0xffffffffu, bar_wait(slot_read + 8 * slot, at_slot.phase ^ 1, gave_up));
                 if (!ok) break;
 #pragma unroll
                 for (int a = 0; a < S::kAhead; ++a)
@@ -327,7 +329,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                 if (lane < S::kTileBlocks * S::kAhead) {
                     const int a = lane % S::kAhead;
                     const bool in = kb + a < kb1;
-                    const int64_t wb = min(wb0 + lane / S::kAhead, p.w.row_blocks - 1);
+                    const int64_t wb = min((int64_t(tile.w) * S::kOutputs + (S::SWAP ? 0 : lane / S::kAhead * S::kCols)) / 128, p.w.row_blocks - 1);
                     copy_word_async(at + (S::kAhead * S::kTileRows + lane) * 4, in ? p.w.scales + tile.x * p.w.sms + wb * p.w.srs + (kb + a) * p.w.scs : p.w.scales, in);
                 }
                 bar_arrive_copies(slot_full + 8 * slot);
@@ -340,30 +342,27 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         constexpr int kCols = S::kCols;
         const int quarter = warp & 3, col0 = warp / 4 * kCols;
         const uint32_t my_tmem = tmem + (uint32_t(quarter) << 21) + col0;
-        uint32_t it = 0, chunk = 0;
+        RingAt<NBUF> at_sum;
+        RingAt<S::kSlots> at_slot;
         bool ok = true;
         while (ok && next_tile()) {
             uint64_t acc[kCols / 2];
 #pragma unroll
             for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
             const float* const my_scale = scales + (S::SWAP ? col0 : quarter * 32 + lane);
-            const float* const my_weight = scales + S::kAhead * S::kTileRows + (S::SWAP ? 0 : col0 / 128 * S::kAhead);
+            const float* const my_weight = scales + S::kAhead * S::kTileRows + (S::SWAP ? 0 : warp / 4 * S::kAhead);
             // The waits' results are looked at once per tile: a warp that only goes on after all of its lanes have agreed
             // lost 80 cycles per column block.
-            for (int kb = kb0; kb < kb1; ++kb, ++it) {
-                const int a = (kb - kb0) % S::kAhead;
-                const uint32_t slot = chunk % S::kSlots, b = it % NBUF;
-                if (a == 0) bar_wait(slot_full + 8 * slot, (chunk / S::kSlots) & 1, gave_up);
-                const float* const sx = my_scale + slot * (S::kSlotBytes / 4) + a * S::kTileRows;
-                float scale = my_weight[slot * (S::kSlotBytes / 4) + a];
+            for (int kb = kb0; kb < kb1; kb += S::kAhead, at_slot.next()) {
+              bar_wait(slot_full + 8 * at_slot.i, at_slot.phase, gave_up);
+              const float* sx = my_scale + at_slot.i * (S::kSlotBytes / 4);
+              const float* sw = my_weight + at_slot.i * (S::kSlotBytes / 4);
+              for (int left = min(S::kAhead, kb1 - kb); left > 0; --left, sx += S::kTileRows, ++sw, at_sum.next()) {
+                const uint32_t b = at_sum.i;
+                float scale = *sw;
                 if (!S::SWAP) scale = __fmul_rn(*sx, scale);
                 const uint64_t s2 = pack2(__float_as_uint(scale), __float_as_uint(scale));
-                const bool last = a == S::kAhead - 1 || kb + 1 == kb1;  // of its slot
-                if (!S::SWAP && last) {
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(slot_read + 8 * slot);
-                }
-                bar_wait(done + 8 * b, (it / NBUF) & 1, gave_up);
+                bar_wait(done + 8 * b, at_sum.phase, gave_up);
                 __syncwarp();
                 tc_fence_after();
                 uint32_t v[2][S::LOAD];  // one part being multiplied, the next one on its way
@@ -376,10 +375,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                     if (c + S::LOAD == kCols) {  // all of it is in registers: the accumulator may be written again
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) {
-                            if constexpr (S::PAIR) bar_arrive_remote(bar_at_rank(taken + 8 * b, 0));
-                            else bar_arrive(taken + 8 * b);
-                        }
+                        if (lane == 0) bar_arrive(taken + 8 * b);
                     }
                     if constexpr (S::SWAP) {
 #pragma unroll
@@ -393,17 +389,15 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
                         for (int i = 0; i < S::LOAD; i += 2) fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), s2);
                     }
                 }
-                if (S::SWAP && last) {
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(slot_read + 8 * slot);
-                }
-                if (last) ++chunk;
+              }
+              __syncwarp();
+              if (lane == 0) bar_arrive(slot_read + 8 * at_slot.i);
             }
             ok = !__any_sync(0xffffffffu, *gave_up);
             if (!ok) break;
             const int here = tile.z - tile.y;
             if constexpr (!S::SWAP) {
-                const int m = tile.y + int(half) * 128 + quarter * 32, n = tile.w * S::kOutputs + col0;
+                const int m = tile.y + quarter * 32, n = tile.w * S::kOutputs + col0;
                 if (m < tile.z && n < p.w.rows)
                     store_rows<T, kCols>(extra + warp * 4096, static_cast<T*>(p.out) + m * p.out_ld + n, p.out_ld, acc, min(32, tile.z - m),
                                          int(min(int64_t(kCols), p.w.rows - n)), lane);
@@ -467,18 +461,13 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (S::PAIR) cluster_sync();  // both CTAs have read their accumulators
-    if (warp == S::kIssue) tmem_free<S::PAIR>(tmem, S::kTmem);
+    if (warp == S::kIssue) tmem_free(tmem, S::kTmem);
     if (threadIdx.x == 0 && *gave_up) set_flag(flags, VF_FLAG_GAVE_UP);
     __syncwarp();
     // no CTA ends while another one may still write to it
-    if (S::PAIR) {
-        cluster_sync();
-    } else {
-        if (!joined) cluster_wait();
-        if (!left) cluster_arrive_relaxed();
-        if (in_cluster) cluster_wait();
-    }
+    if (!joined) cluster_wait();
+    if (!left) cluster_arrive_relaxed();
+    if (in_cluster) cluster_wait();
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
@@ -521,7 +510,6 @@ bool fits_bulk_copies(const Blocks& b) {  // start and pitches of 16-byte units,
 
 template <class S, class T>
 void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
-    if (S::PAIR) ranks = 2;
     auto kernel = k_matmul_blocks<S, T>;
     static std::atomic<uint64_t> ready{0};  // devices (below 64) on which this kernel has been set up
     const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
@@ -549,18 +537,18 @@ void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    const uint32_t idesc = tc_f8_shape((S::SWAP ? p.w : p.x).dtype == VF_DT_F8E5M2, (S::SWAP ? p.x : p.w).dtype == VF_DT_F8E5M2, S::PAIR ? 256 : 128, S::BN);
-    VF_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_codes(p.x, 2, S::PAIR ? 128 : S::kTokens), map_codes(p.w, 3, S::SWAP ? 128 : S::kRowsB), p, int(n_tiles), idesc, ctx->d_flags));
+    const uint32_t idesc = tc_f8_shape((S::SWAP ? p.w : p.x).dtype == VF_DT_F8E5M2, (S::SWAP ? p.x : p.w).dtype == VF_DT_F8E5M2, S::BN);
+    VF_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_codes(p.x, 2, S::kTokens), map_codes(p.w, 3, S::kOutputs), p, int(n_tiles), idesc, ctx->d_flags));
 }
 
 //                       BN, stages, accumulators, epilogue groups of four warps, CTAs per SM
-using Swap16 = Shape<Form::kSwap, 16, 5, 4, 1, 2, 16>;
-using Swap32 = Shape<Form::kSwap, 32, 4, 4, 1, 2, 16>;
-using Swap64 = Shape<Form::kSwap, 64, 3, 4, 1, 2, 16>;
-using Swap128 = Shape<Form::kSwap, 128, 4, 2, 2, 1, 16>;
-using Single64 = Shape<Form::kSingle, 64, 3, 4, 1, 2>;
-using Single128 = Shape<Form::kSingle, 128, 5, 2, 2, 1>;
-using Pair256 = Shape<Form::kPair, 256, 5, 2, 2, 1, 16>;
+using Swap16 = Shape<true, 16, 5, 4, 1, 2, 16>;
+using Swap32 = Shape<true, 32, 4, 4, 1, 2, 16>;
+using Swap64 = Shape<true, 64, 3, 4, 1, 2, 16>;
+using Swap128 = Shape<true, 128, 4, 2, 2, 1, 16>;
+using Single64 = Shape<false, 64, 3, 4, 1, 2>;
+using Single128 = Shape<false, 128, 5, 2, 2, 1>;
+using Single256 = Shape<false, 256, 3, 2, 2, 1, 16>;
 
 // CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column blocks
 // that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs about as much as
@@ -598,7 +586,7 @@ void launch_for(vf_ctx* ctx, const BlockProduct& p) {
     } else if (most_row_tiles(p, 128) * n_tiles * 2 <= ctx->sm_count) {
         launch_swapped<Swap128, T>(ctx, p);
     } else {
-        if (most_row_tiles(p, 256) * ((p.w.rows + 255) / 256) >= ctx->sm_count / 2) launch_tensor<Pair256, T>(ctx, p);
+        if (most_row_tiles(p, 128) * ((p.w.rows + 255) / 256) >= ctx->sm_count) launch_tensor<Single256, T>(ctx, p);
         else if (most_row_tiles(p, 128) * n_tiles >= ctx->sm_count) launch_tensor<Single128, T>(ctx, p);
         else launch_tensor<Single64, T>(ctx, p);
     }

@@ -34,16 +34,6 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ uint32_t bar_at_rank(uint32_t bar, uint32_t rank) {  // the same barrier of another CTA of the cluster
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(bar), "r"(rank));
-    return a;
-}
-// arrives at the barrier with the cluster address `bar`, for what tensor memory holds: no writes of this thread have to be
-// visible to the other CTA (a release to the whole cluster waits for all of them and took a microsecond)
-__device__ __forceinline__ void bar_arrive_remote(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
@@ -92,9 +82,6 @@ __device__ __forceinline__ uint32_t cluster_size() {
     asm volatile("mov.u32 %0, %cluster_nctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void cluster_arrive() {  // its wait orders the barriers that were initialised before
     asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
 }
@@ -130,26 +117,13 @@ __device__ __forceinline__ void copies_wait_all() {
 __device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
 }
-// `bar` belongs to this CTA, or (Pair) to either CTA of the pair: an address from bar_at_rank()
-template <bool Pair>
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y) {
-    if constexpr (Pair)
-        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-                     "l"(m), "r"(bar), "r"(x), "r"(y)
-                     : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m), "r"(bar),
+    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst), "l"(m), "r"(bar),
                      "r"(x), "r"(y)
                      : "memory");
 }
-template <bool Pair>
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* m, uint32_t bar, int x, int y, int z) {
-    if constexpr (Pair)
-        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
-                     "l"(m), "r"(bar), "r"(x), "r"(y), "r"(z)
-                     : "memory");
-    else
-        asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(m),
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(m),
                      "r"(bar), "r"(x), "r"(y), "r"(z)
                      : "memory");
 }
@@ -159,21 +133,12 @@ __device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* m, int x, int
 }
 
 // ---- tensor core -------------------------------------------------------------------------------------------------------
-// Pair: the two CTAs of a pair (cluster ranks 2i and 2i + 1) work on one tile. Both allocate and free, the even one issues.
-template <bool Pair>
 __device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t columns) {  // one whole warp
-    if constexpr (Pair) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-    } else {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-template <bool Pair>
 __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {  // the warp that allocated
-    if constexpr (Pair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
+ asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() {
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -181,27 +146,14 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-// arrives at `bar` (Pair: of both CTAs) once every tensor-core operation that this thread has issued is complete
-template <bool Pair>
+// arrives at `bar` once every tensor-core operation that this thread has issued is complete
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-    if constexpr (Pair)
-        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(uint16_t(3))
-                     : "memory");
-    else
-        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// D[128 x N] (+)= A[128 x 32] * B[N x 32]^T, 8-bit floats in shared memory, fp32 in tensor memory. Pair: D and A have 256 rows,
-// 128 in each CTA, and each CTA holds half of B's rows.
-template <bool Pair>
+// D[128 x N] (+)= A[128 x 32] * B[N x 32]^T, 8-bit floats in shared memory, fp32 in tensor memory.
 __device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-    if constexpr (Pair)
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
-            "r"(idesc), "r"(uint32_t(accumulate))
-            : "memory");
-    else
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
             "r"(idesc), "r"(uint32_t(accumulate))
             : "memory");
 }
@@ -210,9 +162,9 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d, uint64_t a, uint64_t b, ui
 __device__ __forceinline__ uint64_t tc_operand(uint32_t addr) {
     return uint64_t((addr >> 4) & 0x3FFFu) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
-// Instruction descriptor of kind::f8f6f4: fp32 result, both operands K-major
-__host__ __device__ inline uint32_t tc_f8_shape(bool a_e5m2, bool b_e5m2, int m, int n) {
-    return (1u << 4) | (uint32_t(a_e5m2) << 7) | (uint32_t(b_e5m2) << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
+// Instruction descriptor of kind::f8f6f4: fp32 result, both operands K-major, M = 128
+__host__ __device__ inline uint32_t tc_f8_shape(bool a_e5m2, bool b_e5m2, int n) {
+    return (1u << 4) | (uint32_t(a_e5m2) << 7) | (uint32_t(b_e5m2) << 10) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
 }
 // 16 consecutive columns of this warp's 32 lanes (one lane per thread)
 __device__ __forceinline__ void tmem_load(uint32_t (&v)[16], uint32_t addr) {
