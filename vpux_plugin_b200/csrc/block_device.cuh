@@ -56,7 +56,7 @@ __device__ __forceinline__ __nv_bfloat16 to_wide<__nv_bfloat16>(float v) {
 // Walks the tiles of a product in ascending order. A tile is `bm` rows of one expert by one of `n_tiles` column tiles;
 // the tiles of expert e come before those of e + 1, and within an expert the row tiles of a column tile follow one
 // another, so that tiles which run at the same time share the weights. Without offsets all rows form one group. Every method is
-// called by whole warps. Offsets are read 32 at a time, one expert per lane; they are clamped into the operand, and
+// called by whole warps; the number of tiles fits 32 bits (most_tiles() sees to it). Offsets are read 32 at a time, one expert per lane; they are clamped into the operand, and
 // offsets that had to be clamped set a flag.
 struct TileWalk {
     const int64_t* offsets;
@@ -64,8 +64,8 @@ struct TileWalk {
     int experts, bm, n_tiles;
     int64_t rows;
     int e0;                // expert of lane 0
-    int64_t base;          // tiles before expert e0
-    int64_t through;       // tiles of experts e0 .. e0 + lane
+    int base;              // tiles before expert e0
+    int through;           // tiles of experts e0 .. e0 + lane
     int lo, hi;            // this lane's rows
     // the tile found
     int expert, row0, row_end, n_tile;
@@ -80,10 +80,10 @@ struct TileWalk {
             lo = int(ca);
             hi = int(cb);
         }
-        through = int64_t((hi - lo + bm - 1) / bm) * n_tiles;
+        through = int(uint32_t(hi - lo + bm - 1) / uint32_t(bm)) * n_tiles;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int64_t o = __shfl_up_sync(0xffffffffu, through, d);
+            const int o = __shfl_up_sync(0xffffffffu, through, d);
             if (int(threadIdx.x & 31) >= d) through += o;
         }
     }
@@ -99,18 +99,18 @@ struct TileWalk {
         if (offsets) load();
     }
     // Finds tile `t` (not below the one found before); false behind the last tile.
-    __device__ __forceinline__ bool find(int64_t t) {
+    __device__ __forceinline__ bool find(int t) {
         if (!offsets) {  // one group: nothing to search
             const int m_tiles = (int(rows) + bm - 1) / bm;
-            if (t >= int64_t(m_tiles) * n_tiles) return false;
+            if (t >= m_tiles * n_tiles) return false;
             n_tile = int(uint32_t(t) / uint32_t(m_tiles));
             expert = 0;
-            row0 = (int(t) - n_tile * m_tiles) * bm;
+            row0 = (t - n_tile * m_tiles) * bm;
             row_end = int(rows);
             return true;
         }
         for (;;) {
-            const int64_t here = __shfl_sync(0xffffffffu, through, 31);
+            const int here = __shfl_sync(0xffffffffu, through, 31);
             if (t - base < here) break;
             base += here;
             e0 += 32;
@@ -121,13 +121,13 @@ struct TileWalk {
             }
             load();
         }
-        const int64_t rel = t - base;
+        const int rel = t - base;
         const int src = __ffs(__ballot_sync(0xffffffffu, through > rel)) - 1;
         const int l = __shfl_sync(0xffffffffu, lo, src), h = __shfl_sync(0xffffffffu, hi, src);
-        const int64_t before = src ? __shfl_sync(0xffffffffu, through, src ? src - 1 : 0) : 0;
-        const int m_tiles = (h - l + bm - 1) / bm;
-        const int in_expert = int(rel - before);
-        n_tile = in_expert / m_tiles;
+        const int before = __shfl_sync(0xffffffffu, through, src ? src - 1 : 0);
+        const int m_tiles = int(uint32_t(h - l + bm - 1) / uint32_t(bm));
+        const int in_expert = src ? rel - before : rel;
+        n_tile = int(uint32_t(in_expert) / uint32_t(m_tiles));
         expert = e0 + src;
         row0 = l + (in_expert - n_tile * m_tiles) * bm;
         row_end = h;

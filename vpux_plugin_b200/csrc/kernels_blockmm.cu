@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(256) k_matmul_blocks_plain(BlockProduct p, int
     walk.start(p.offsets, p.offsets ? int(p.w.count) : 1, p.x.rows, kPlain, n_tiles, flags);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
     const bool x5 = p.x.dtype == VF_DT_F8E5M2, w5 = p.w.dtype == VF_DT_F8E5M2;
-    for (int64_t t = blockIdx.x; walk.find(t); t += gridDim.x) {
+    for (int t = blockIdx.x; walk.find(t); t += gridDim.x) {
         const int m0 = walk.row0, m_end = walk.row_end, n0 = walk.n_tile * kPlain;
         const uint8_t* w = p.w.codes + walk.expert * p.w.matrix_stride;
         const float* wscale = p.w.scales + walk.expert * p.w.sms + (n0 / kBlock) * p.w.srs;
@@ -71,10 +71,18 @@ int64_t most_row_tiles(const BlockProduct& p, int bm) {
     return p.offsets ? std::min(p.x.rows, whole + p.w.count) : whole;
 }
 
+// Tiles of bm rows by bn columns, as an upper bound. The kernels count them (and one step of their grid) in 32 bits: a result
+// with so many tiles does not fit the device's memory, a claim of one is refused.
+int64_t most_tiles(const BlockProduct& p, int bm, int bn) {
+    const int64_t rows = most_row_tiles(p, bm), cols = (p.w.rows + bn - 1) / bn;
+    if (rows > (int64_t(1) << 30) / cols) raise(VF_ERR_CAPACITY, "a product of %lld by %lld tiles", (long long)rows, (long long)cols);
+    return rows * cols;
+}
+
 template <class T>
 void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
     const int64_t n_tiles = (p.w.rows + kPlain - 1) / kPlain;
-    const int64_t tiles = most_row_tiles(p, kPlain) * n_tiles;
+    const int64_t tiles = most_tiles(p, kPlain, kPlain);
     k_matmul_blocks_plain<T><<<unsigned(std::min<int64_t>(tiles, 8 * ctx->sm_count)), 256, 0, ctx->stream>>>(p, int(n_tiles), ctx->d_flags);
 }
 
@@ -252,7 +260,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
         uint32_t it = 0;
         RingAt<STAGES> at_stage;
         bool ok = true;
-        for (int64_t t = blockIdx.x / ranks; ok; t += gridDim.x / ranks, ++turn) {
+        for (int t = blockIdx.x / ranks; ok; t += gridDim.x / ranks, ++turn) {
             const bool more = walk.find(t);
             const uint32_t i = turn & 1;
             ok = __all_sync(0xffffffffu, bar_wait(tile_read + 8 * i, ((turn >> 1) & 1) ^ 1, gave_up));
@@ -523,7 +531,7 @@ void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
         ready.fetch_or(bit, std::memory_order_relaxed);
     }
     const int64_t n_tiles = (p.w.rows + S::kOutputs - 1) / S::kOutputs;
-    const int64_t tiles = most_row_tiles(p, S::kTokens) * n_tiles;
+    const int64_t tiles = most_tiles(p, S::kTokens, S::kOutputs);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned((S::SWAP && ranks > 1 ? tiles : std::min<int64_t>(tiles, ctx->sm_count * S::PER_SM / ranks)) * ranks));
     cfg.blockDim = dim3(S::kThreads);
@@ -569,7 +577,7 @@ int ranks_for(vf_ctx* ctx, int64_t tiles, int64_t col_blocks) {
 
 template <class S, class T>
 void launch_swapped(vf_ctx* ctx, const BlockProduct& p) {
-    launch_tensor<S, T>(ctx, p, ranks_for<S>(ctx, most_row_tiles(p, S::BN) * ((p.w.rows + 127) / 128), p.x.col_blocks));
+    launch_tensor<S, T>(ctx, p, ranks_for<S>(ctx, most_tiles(p, S::BN, 128), p.x.col_blocks));
 }
 
 template <class T>
@@ -583,11 +591,11 @@ void launch_for(vf_ctx* ctx, const BlockProduct& p) {
         launch_swapped<Swap32, T>(ctx, p);
     } else if (rows <= 64) {
         launch_swapped<Swap64, T>(ctx, p);
-    } else if (most_row_tiles(p, 128) * n_tiles * 2 <= ctx->sm_count) {
+    } else if (most_tiles(p, 128, 128) * 2 <= ctx->sm_count) {
         launch_swapped<Swap128, T>(ctx, p);
     } else {
-        if (most_row_tiles(p, 128) * ((p.w.rows + 255) / 256) >= ctx->sm_count) launch_tensor<Single256, T>(ctx, p);
-        else if (most_row_tiles(p, 128) * n_tiles >= ctx->sm_count) launch_tensor<Single128, T>(ctx, p);
+        if (most_tiles(p, 128, 256) >= ctx->sm_count) launch_tensor<Single256, T>(ctx, p);
+        else if (most_tiles(p, 128, 128) >= ctx->sm_count) launch_tensor<Single128, T>(ctx, p);
         else launch_tensor<Single64, T>(ctx, p);
     }
 }
