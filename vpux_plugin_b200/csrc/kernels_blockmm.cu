@@ -517,87 +517,100 @@ bool fits_bulk_copies(const Blocks& b) {  // start and pitches of 16-byte units,
 }
 
 template <class S, class T>
-void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
-    auto kernel = k_matmul_blocks<S, T>;
-    static std::atomic<uint64_t> ready{0};  // devices (below 64) on which this kernel has been set up
-    const uint64_t bit = ctx->device < 64 ? uint64_t(1) << ctx->device : 0;
-    if (!(ready.load(std::memory_order_relaxed) & bit)) {
+struct Kernel {
+    static constexpr int kDevices = 64;
+    static cudaLaunchConfig_t config(cudaLaunchAttribute (&attr)[2], int64_t ctas, int ranks, cudaStream_t st) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(unsigned(ctas));
+        cfg.blockDim = dim3(S::kThreads);
+        cfg.dynamicSmemBytes = S::kSmem;
+        cfg.stream = st;
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = unsigned(ranks);
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (see chain_enter)
+        attr[1].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 2;
+        return cfg;
+    }
+    static void prepare(vf_ctx* ctx) {  // what a device has to be told once
+        static std::atomic<bool> ready[kDevices];
+        if (ctx->device < kDevices && ready[ctx->device].load(std::memory_order_acquire)) return;
+        auto kernel = k_matmul_blocks<S, T>;
         VF_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
         if (S::kTrades) {  // warps that take registers wait until they are there: what is taken has to have been given
             cudaFuncAttributes fa;
             VF_CUDA(cudaFuncGetAttributes(&fa, kernel));
             if (fa.numRegs * S::kThreads < 128 * kGiven + 128 * S::GROUPS * kTaken) raise(VF_ERR_CUDA, "the kernel was built with too few registers");
         }
-        ready.fetch_or(bit, std::memory_order_relaxed);
+        if (ctx->device < kDevices) ready[ctx->device].store(true, std::memory_order_release);
     }
+};
+
+template <class S, class T>
+void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
+    Kernel<S, T>::prepare(ctx);
     const int64_t n_tiles = (p.w.rows + S::kOutputs - 1) / S::kOutputs;
     const int64_t tiles = most_tiles(p, S::kTokens, S::kOutputs);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(unsigned((S::SWAP && ranks > 1 ? tiles : std::min<int64_t>(tiles, ctx->sm_count * S::PER_SM / ranks)) * ranks));
-    cfg.blockDim = dim3(S::kThreads);
-    cfg.dynamicSmemBytes = S::kSmem;
-    cfg.stream = ctx->stream;
+    const int64_t clusters = S::SWAP && ranks > 1 ? tiles : std::min<int64_t>(tiles, ctx->sm_count * S::PER_SM);
     cudaLaunchAttribute attr[2] = {};
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // (see chain_enter)
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = unsigned(ranks);
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    const cudaLaunchConfig_t cfg = Kernel<S, T>::config(attr, clusters * ranks, ranks, ctx->stream);
     const uint32_t idesc = tc_f8_shape((S::SWAP ? p.w : p.x).dtype == VF_DT_F8E5M2, (S::SWAP ? p.x : p.w).dtype == VF_DT_F8E5M2, S::BN);
-    VF_CUDA(cudaLaunchKernelEx(&cfg, kernel, map_codes(p.x, 2, S::kTokens), map_codes(p.w, 3, S::kOutputs), p, int(n_tiles), idesc, ctx->d_flags));
+    VF_CUDA(cudaLaunchKernelEx(&cfg, k_matmul_blocks<S, T>, map_codes(p.x, 2, S::kTokens), map_codes(p.w, 3, S::kOutputs), p, int(n_tiles), idesc, ctx->d_flags));
 }
 
-//                       BN, stages, accumulators, epilogue groups of four warps, CTAs per SM
+//                    BN, stages, accumulators, epilogue groups of four warps, CTAs per SM, columns per load
 using Swap16 = Shape<true, 16, 5, 4, 1, 2, 16>;
 using Swap32 = Shape<true, 32, 4, 4, 1, 2, 16>;
 using Swap64 = Shape<true, 64, 3, 4, 1, 2, 16>;
 using Swap128 = Shape<true, 128, 4, 2, 2, 1, 16>;
-using Single64 = Shape<false, 64, 3, 4, 1, 2>;
-using Single128 = Shape<false, 128, 5, 2, 2, 1>;
-using Single256 = Shape<false, 256, 3, 2, 2, 1, 16>;
+using Wide128 = Shape<false, 128, 5, 2, 2, 1, 32>;
+using Wide256 = Shape<false, 256, 3, 2, 2, 1, 16>;
 
-// CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column blocks
-// that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs about as much as
-// four of them. (48 rows, 4096 x 11008, 32 tiles of 86 blocks: 18.7 us with four, 13.5 with eight.)
-template <class S>
-int ranks_for(vf_ctx* ctx, int64_t tiles, int64_t col_blocks) {
+// Few rows: CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column
+// blocks that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs
+// about as much as four of them. (48 rows, 4096 x 11008, 32 tiles of 86 blocks: 40 us alone, 18.7 with four, 13.7 with eight, although
+// the last of 32 such clusters has to wait for a place. Clusters of eight CTAs with a multiprocessor each wait more
+// often: [256, 1024, 8192] in 19.6 us with eight, 15.5 with four.)
+template <class S, class T>
+void launch_swapped(vf_ctx* ctx, const BlockProduct& p) {
+    const int64_t tiles = most_tiles(p, S::BN, 128);
     int best = 1;
-    int64_t least = col_blocks;
-    for (int r = 2; r <= 8 && tiles * r <= S::PER_SM * ctx->sm_count && 2 * r <= col_blocks; ++r) {
-        const int64_t load = (col_blocks + r - 1) / r + 4;
+    int64_t least = p.x.col_blocks;
+    for (int r = 2; r <= 4 * S::PER_SM && 2 * r <= p.x.col_blocks && tiles * r <= S::PER_SM * ctx->sm_count; ++r) {
+        const int64_t load = (p.x.col_blocks + r - 1) / r + 4;
         if ((S::kFours + r - 1) / r * r <= S::kParts && load < least) {
             least = load;
             best = r;
         }
     }
-    return best;
+    launch_tensor<S, T>(ctx, p, best);
 }
 
-template <class S, class T>
-void launch_swapped(vf_ctx* ctx, const BlockProduct& p) {
-    launch_tensor<S, T>(ctx, p, ranks_for<S>(ctx, most_tiles(p, S::BN, 128), p.x.col_blocks));
-}
-
+// The form goes by the rows of activations (of an expert, on average). Times in us, [rows, outputs, columns]:
+//   up to 16      [16, 4096, 4096]    Swap16 6.7   Swap32 7.0   Swap64 8.5
+//   up to 32      [32, 11008, 4096]   Swap16 15.8  Swap32 12.2  Swap64 15.7
+//   up to 64      [33, 11008, 4096]   Swap32 17.2  Swap64 15.9  Swap128 18.6; grouped, 57 rows on average, 16 experts [2048, 2048]:
+//                 Swap32 19.9  Swap64 26.1  Swap128 23.5, since most experts' rows end inside a tile
+//   above, where tiles of 128 x 128 leave half of the multiprocessors idle, Swap128 splits them:
+//                 [128, 4096, 4096]   Swap128 10.9  Wide128 15.3  Wide256 17.6; [192, 4096, 4096] (64 tiles) 14.5, 15.6, 17.8
+//   else by the rounds that the tiles take; one of Wide256's takes 1.2 times as long as one of Wide128's:
+//                 [512, 4096, 4096]   128 or 64 tiles, one round either way: Wide128 16.2  Wide256 18.8
+//                 [1024, 4096, 4096]  256 or 128 tiles, two rounds or one: Wide128 29.1  Wide256 20.5
 template <class T>
 void launch_for(vf_ctx* ctx, const BlockProduct& p) {
     if (!fits_bulk_copies(p.x) || !fits_bulk_copies(p.w)) return launch_plain<T>(ctx, p);
     const int64_t rows = p.offsets ? (p.x.rows + p.w.count - 1) / p.w.count : p.x.rows;
-    const int64_t n_tiles = (p.w.rows + 127) / 128;
-    if (rows <= 16) {
-        launch_swapped<Swap16, T>(ctx, p);
-    } else if (rows <= 32) {
-        launch_swapped<Swap32, T>(ctx, p);
-    } else if (rows <= 64) {
-        launch_swapped<Swap64, T>(ctx, p);
-    } else if (most_tiles(p, 128, 128) * 2 <= ctx->sm_count) {
-        launch_swapped<Swap128, T>(ctx, p);
-    } else {
-        if (most_tiles(p, 128, 256) >= ctx->sm_count) launch_tensor<Single256, T>(ctx, p);
-        else if (most_tiles(p, 128, 128) >= ctx->sm_count) launch_tensor<Single128, T>(ctx, p);
-        else launch_tensor<Single64, T>(ctx, p);
-    }
+    if (rows <= 16) return launch_swapped<Swap16, T>(ctx, p);
+    if (rows <= 32 || (p.offsets && rows <= 64)) return launch_swapped<Swap32, T>(ctx, p);
+    if (rows <= 64) return launch_swapped<Swap64, T>(ctx, p);
+    // (of the experts' last tiles, half are counted: the bound that the grid is sized by counts one for every expert)
+    const int64_t row_tiles = (p.x.rows + 127) / 128 + (p.offsets ? p.w.count / 2 : 0), sms = ctx->sm_count;
+    const int64_t few = row_tiles * ((p.w.rows + 127) / 128), wide = row_tiles * ((p.w.rows + 255) / 256);
+    if (few * 2 <= sms) return launch_swapped<Swap128, T>(ctx, p);
+    if ((wide + sms - 1) / sms * 12 < (few + sms - 1) / sms * 10) return launch_tensor<Wide256, T>(ctx, p);
+    launch_tensor<Wide128, T>(ctx, p);
 }
 
 }  // namespace
