@@ -324,6 +324,110 @@ def test_grouped_product_with_many_tiles(gpu, torch, offsets, n):
     assert (got[:offsets[0]] == 3).all() and (got[offsets[-1]:] == 3).all()
 
 
+@pytest.mark.parametrize("k", [257, 640, 1153, 2100, 4480])
+@pytest.mark.parametrize("m", [1, 5, 16, 17, 30, 33, 50, 64, 66, 100, 128, 140, 250])
+def test_product_of_few_rows_and_long_sums(gpu, torch, m, k):
+    """Column blocks that two to eight CTAs share, in numbers that do not divide evenly."""
+    rng = np.random.default_rng(26)
+    for n in (120, 300):
+        ops = operands(rng, m, n, k, E4M3, E4M3)
+        got = run_product(gpu, torch, *ops, E4M3, E4M3, F32)
+        check_product(got, *ops, E4M3, E4M3, F32)
+
+
+def test_elements_beyond_32_bits(gpu, torch):
+    """Matrices of more than 2^31 elements: the last rows of quantising, reading back and both products."""
+    rng = np.random.default_rng(27)
+    rows, cols = 70000, 32000
+    src = torch.zeros(rows * cols, dtype=torch.bfloat16, device="cuda").view(rows, cols)
+    x = host_f32(torch, weight_values(rng, (130, cols)), BF16)
+    src[-130:] = torch.from_numpy(x).to(torch.bfloat16)
+    codes = torch.full((rows, cols), GUARD, dtype=torch.uint8, device="cuda")
+    for block_rows in (1, 128):
+        scales = torch.zeros(-(-rows // block_rows), 250, device="cuda")
+        m = abi.block_matrix(codes.data_ptr(), scales.data_ptr(), E4M3, block_rows, rows, cols)
+        c, keep = device_content(torch, src, BF16, (rows, cols))
+        torch.cuda.synchronize()
+        gpu.quantize_blocks(c, m)
+        first = rows - 130 if block_rows == 1 else rows // 128 * 128  # the first row of a whole block of known values
+        want_c, want_s = br.quantize(x[first - (rows - 130):], block_rows, E4M3)
+        assert np.array_equal(codes[first:].cpu().numpy(), want_c)
+        assert np.array_equal(scales[first // block_rows:].cpu().numpy(), want_s)
+        codes[:1000] = 7
+        src[:1000] = 0
+        torch.cuda.synchronize()
+        gpu.dequantize_blocks(m, src.data_ptr(), BF16, src.nbytes)
+        want = rounded(torch, br.values(want_c, want_s, block_rows, E4M3), BF16)
+        assert np.array_equal(src[first:].float().cpu().numpy(), want)
+        src[-130:] = torch.from_numpy(x).to(torch.bfloat16)
+    # results beyond 2^31 elements, and weights of as many codes (the last of nine experts)
+    xc, xs = br.quantize(rng.standard_normal((rows, 16)).astype(np.float32), 1, E4M3)
+    wc, ws = br.quantize(weight_values(rng, (cols, 16)), 128, E4M3)
+    xm, wm = Matrix(torch, rows, 16, 1, codes=xc, scales=xs), Matrix(torch, cols, 16, 128, codes=wc, scales=ws)
+    gpu.matmul_blocks(xm.pod, wm.pod, src.data_ptr(), BF16, src.nbytes)
+    part = (xc[-40:], xs[-40:], wc[None], ws[None])
+    check_product(src[-40:].double().cpu().numpy(), *part, E4M3, E4M3, BF16)
+    del src
+    experts, n, k = 9, 16384, 16384
+    big = codes.view(-1)[:0].new_empty(experts * n * k)
+    big.fill_(0)
+    wc, ws = br.quantize(weight_values(rng, (1, 256, k)), 128, E4M3)
+    big.view(experts, n, k)[-1, -256:] = torch.from_numpy(wc[0])
+    all_s = torch.ones(experts, n // 128, k // 128, device="cuda")
+    all_s[-1, -2:] = torch.from_numpy(ws[0])
+    wm = abi.block_matrix(big.data_ptr(), all_s.data_ptr(), E4M3, 128, n, k, count=experts)
+    xc, xs = br.quantize(rng.standard_normal((12, k)).astype(np.float32), 1, E4M3)
+    xm = Matrix(torch, 12, k, 1, codes=xc, scales=xs)
+    offs = torch.tensor([0] * 4 + [5] * 5 + [12], device="cuda")
+    out = torch.zeros(12, n, device="cuda")
+    torch.cuda.synchronize()
+    gpu.matmul_blocks_grouped(xm.pod, wm, offs.data_ptr(), out.data_ptr(), F32, out.nbytes)
+    check_product(out[:, -256:].double().cpu().numpy(), xc, xs, wc, ws, E4M3, E4M3, F32, 5, 12)
+    assert (out[:5] == 0).all() and (out[5:, :-256] == 0).all()
+
+
+def test_a_claim_of_more_tiles_than_fit_is_refused(gpu):
+    at = 1 << 40  # addresses that nothing looks at
+    x = abi.block_matrix(at, 2 * at, E4M3, 1, 1 << 30, 16)
+    w = abi.block_matrix(3 * at, 4 * at, E4M3, 128, 1 << 21, 16)
+    with pytest.raises(VfoldError) as e:
+        gpu.matmul_blocks(x, w, 1 << 60, BF16, 1 << 59)
+    assert e.value.status == abi.VF_ERR_CAPACITY
+
+
+def test_memory_kinds_mixed(gpu, torch):
+    rng = np.random.default_rng(28)
+    x = weight_values(rng, (40, 300))
+    codes, scales = br.quantize(x, 1, E4M3)
+    m = Matrix(torch, 40, 300, 1)
+    c, keep = abi.make_content(abi.TType([40, 300], F32), x)  # from host memory to the device
+    gpu.quantize_blocks(c, m.pod)
+    assert np.array_equal(m.codes()[0], codes) and np.array_equal(m.scales()[0], scales)
+    src, k1 = to_device(torch, x, F32)
+    torch.cuda.synchronize()
+    c, k2 = device_content(torch, src, F32, (40, 300))  # and back
+    q, s = np.zeros((40, 300), np.uint8), np.zeros((3, 40), np.float32)
+    gpu.quantize_blocks(c, abi.block_matrix(q, s, E4M3, 1, 40, 300, scale_row_stride=1, scale_col_stride=40, mem_kind=HOST))
+    assert np.array_equal(q, codes) and np.array_equal(s.T, scales)
+    back = np.zeros_like(x)
+    gpu.dequantize_blocks(m.pod, back, F32, back.nbytes, dst_mem_kind=HOST)
+    assert np.array_equal(back, br.values(codes, scales, 1, E4M3).astype(np.float32))
+
+
+def test_on_the_legacy_default_stream(torch):
+    """The handle 1 stands for the default stream, so calls line up with what torch enqueues there."""
+    lib = Library(device=0, stream=1, pipelined=True)
+    rng = np.random.default_rng(29)
+    ops = operands(rng, 20, 300, 512, E4M3, E4M3)
+    x, w = Matrix(torch, 20, 512, 1, codes=ops[0], scales=ops[1]), Matrix(torch, 300, 512, 128, codes=ops[2], scales=ops[3])
+    y = torch.empty(20, 300, device="cuda")
+    y.fill_(3)
+    lib.matmul_blocks(x.pod, w.pod, y.data_ptr(), F32, y.nbytes)
+    doubled = y * 2  # behind the product, without a wait
+    check_product(doubled.double().cpu().numpy() / 2, *ops, E4M3, E4M3, F32)
+    lib.close()
+
+
 @pytest.mark.parametrize("m", [3, 70, 300])
 @pytest.mark.parametrize("x_kw,w_kw,out_ld,out_offset", [
     ({"ld": 320, "col_major": False}, {"ld": 336, "col_major": True}, 0, 0),      # scales in the other orders, rows further apart

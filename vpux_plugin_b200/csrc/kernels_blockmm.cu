@@ -88,18 +88,29 @@ void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
 
 
 // ---- tensor cores ------------------------------------------------------------------------------------------------------
-// The weights are the 128-row operand: a tile holds 128 outputs n (one row block of the weights, hence ONE weight scale
-// per column block) of BN activations m. The products of one column block (four steps of 32 k) start from zero in one of NBUF
-// accumulators in tensor memory; while the tensor core fills the next one, the epilogue warps read it, multiply it by the
-// column block's scales and add it to the running sums, which stay in registers:  sum[m] += part[m] * (sx[m] * sw).
-// With BN = 256 that is 128 sums per thread in 8 warps.
+// One column block is four matrix instructions of 32 k. It starts from zero in one of NBUF accumulators in tensor memory; while
+// the tensor core fills the next one, the epilogue warps read it, multiply it by the column block's scales and add it to the
+// running sums, which stay in registers:   sum += part * (sx * sw)
+// Weights have one scale per 128 rows, activations one per row. That decides which operand is which:
+//   many rows    the 128-row operand is 128 activations, one per thread of a group of four epilogue warps, and a thread multiplies
+//                all of its columns (outputs) by the same number. (With the weights there, a 256-column tile reads 256 scales
+//                per column block and thread from shared memory: [4096, 11008, 4096] 281 us against 228 at that stage.)
+//   few rows     the 128-row operand is 128 outputs, the other one 16 to 128 activations, so that no matrix instruction works on
+//                rows that are not there; the scales are one per column.
+// Few rows make few tiles as well: the column blocks of a tile are then spread over the CTAs of a cluster, which push their sums
+// to each other's shared memory, four columns to the CTA that owns them, where they are added in the order of the ranks.
 //
-// Warps: the first ones are the epilogue, in groups of four that read a quarter of tensor memory's lanes each; then one that
-// copies tiles in (bulk tensor copies into a ring of STAGES) and one that issues the matrix instructions.
+// Warps: the first ones are the epilogue, in groups of four that read a quarter of tensor memory's lanes each; then one that finds
+// tiles and copies them in (bulk tensor copies into a ring of STAGES), one that issues the matrix instructions, and one that
+// brings the scales of eight column blocks at a time into a ring of their own.
 //
-// Few rows make few tiles: the column blocks of a tile are then spread over the CTAs of a cluster, which add up their
-// sums through each other's shared memory, every CTA for its share of the tile's rows of activations, always in the order of
-// the ranks.
+// Measured ([rows, outputs, columns], back to back, graph replay): [4096, 11008, 4096] 180 us, 2.05 PFLOP/s, tensor pipe active 53 %
+// of the time; 912 cycles per column block and tile, of which the tensor core needs 512. What bounds it: two
+// accumulators of 256 columns fill the tensor memory, and from one use of an accumulator to the next pass the instructions (512),
+// the epilogue's 480 cycles of reading it and three hand-overs through barriers; and the power limit (1.6 GHz under this load).
+// Tried: pairs of CTAs (256 x 256 tiles) 177-184 us, 128 x 192 tiles 206, four epilogue groups 193-199, four accumulators of 128
+// columns 227-247, 32 columns per load 190, the column-block loop unrolled twice 221-290 (it spills). [1, 11008, 4096] 10.6 us and
+// [48, 4096, 11008] 13.8 us at 4.3 and 3.3 TB/s of weights; [1, 32000, 8192] 43.4 us at 6.0 TB/s: a launch costs 3.5 us of its own.
 constexpr int kGiven = 72, kTaken = 216;  // registers per thread after the trade: 128 * 72 + 256 * 216 = 384 * 168
 
 template <bool SWAP_, int BN_, int STAGES_, int NBUF_, int GROUPS_, int PER_SM_, int LOAD_ = 32>
@@ -111,7 +122,8 @@ struct Shape {
     static constexpr int kEpilogue = 4 * GROUPS, kCopies = kEpilogue, kIssue = kEpilogue + 1, kScaling = kEpilogue + 2;  // warps
     static constexpr bool kTrades = kCols > 64;             // the warps behind the epilogue's give it registers, as a group of four
     static constexpr int kThreads = 32 * (kEpilogue + (kTrades ? 4 : 3));
-    // scales of kAhead column blocks at a time: [kAhead][kTileRows] of the activations, [kTileBlocks][kAhead] of the weights of an epilogue group's columns
+    // scales of kAhead column blocks at a time: [kAhead][kTileRows] of the activations, then [kTileBlocks][kAhead] of the weights,
+    // one row for each epilogue group's columns
     static constexpr int kAhead = 8, kSlots = 2, kTileRows = SWAP ? BN : 128, kTileBlocks = SWAP ? 1 : GROUPS;
     static constexpr int kSlotBytes = kAhead * (kTileRows + kTileBlocks) * 4;
     static constexpr int kStageBytes = (128 + BN) * kBlock;
@@ -253,98 +265,98 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
     };
 
     if (warp >= S::kEpilogue) {
-    if constexpr (S::kTrades) regs_give<kGiven>();
-    if (warp == S::kCopies) {  // ---- finding tiles, copying them in
-        TileWalk walk;
-        walk.start(p.offsets, p.offsets ? int(p.w.count) : 1, p.x.rows, S::kTokens, n_tiles, flags);
-        uint32_t it = 0;
-        RingAt<STAGES> at_stage;
-        bool ok = true;
-        for (int t = blockIdx.x / ranks; ok; t += gridDim.x / ranks, ++turn) {
-            const bool more = walk.find(t);
-            const uint32_t i = turn & 1;
-            ok = __all_sync(0xffffffffu, bar_wait(tile_read + 8 * i, ((turn >> 1) & 1) ^ 1, gave_up));
-            if (!ok) break;
-            if (lane == 0) {
-                tiles[i] = more ? make_int4(walk.expert, walk.row0, walk.row_end, walk.n_tile) : make_int4(-1, 0, 0, 0);
-                bar_arrive(tile_there + 8 * i);
-            }
-            if (!more) break;
-            for (int kb = kb0; kb < kb1; ++kb, ++it, at_stage.next()) {
-                const uint32_t s = at_stage.i, at = smem_addr(ring) + s * S::kStageBytes;
-                ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, at_stage.phase ^ 1, gave_up));
+        if constexpr (S::kTrades) regs_give<kGiven>();
+        if (warp == S::kCopies) {  // ---- finding tiles, copying them in
+            TileWalk walk;
+            walk.start(p.offsets, p.offsets ? int(p.w.count) : 1, p.x.rows, S::kTokens, n_tiles, flags);
+            uint32_t it = 0;
+            RingAt<STAGES> at_stage;
+            bool ok = true;
+            for (int t = blockIdx.x / ranks; ok; t += gridDim.x / ranks, ++turn) {
+                const bool more = walk.find(t);
+                const uint32_t i = turn & 1;
+                ok = __all_sync(0xffffffffu, bar_wait(tile_read + 8 * i, ((turn >> 1) & 1) ^ 1, gave_up));
                 if (!ok) break;
-                if (elect_one()) {
-                    bar_expect(full + 8 * s, S::kStageBytes);
-                    tma_load_3d(S::SWAP ? at : at + 128 * kBlock, &wmap, full + 8 * s, kb * kBlock, walk.n_tile * S::kOutputs, walk.expert);
-                    tma_load_2d(S::SWAP ? at + 128 * kBlock : at, &xmap, full + 8 * s, kb * kBlock, walk.row0);
+                if (lane == 0) {
+                    tiles[i] = more ? make_int4(walk.expert, walk.row0, walk.row_end, walk.n_tile) : make_int4(-1, 0, 0, 0);
+                    bar_arrive(tile_there + 8 * i);
                 }
-            }
-        }
-        if (ok && lane == 0)  // every arrival at the ring's barriers has happened before the CTA ends
-            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) bar_wait(empty + 8 * (i % STAGES), (i / STAGES) & 1, gave_up);
-        if (!ok && lane == 0)  // the copies in flight land before the CTA ends
-            for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
-                const uint64_t t0 = global_ns();
-                while (!bar_try(full + 8 * (i % STAGES), (i / STAGES) & 1) && global_ns() - t0 < kDrainLimitNs) {
-                }
-            }
-    } else if (warp == S::kIssue) {  // ---- matrix instructions
-        RingAt<STAGES> at_stage;
-        RingAt<NBUF> at_sum;
-        bool ok = true;
-        while (ok && next_tile()) {
-            for (int kb = kb0; kb < kb1; ++kb, at_stage.next(), at_sum.next()) {
-                const uint32_t s = at_stage.i, b = at_sum.i;
-                const uint32_t at = smem_addr(ring) + s * S::kStageBytes;
-                const uint64_t ad = tc_operand(at), bd = tc_operand(at + 128 * kBlock);
-                // the accumulator last: with it the time between two uses of one accumulator starts to run
-                ok = __all_sync(0xffffffffu, bar_wait(full + 8 * s, at_stage.phase, gave_up) && bar_wait(taken + 8 * b, at_sum.phase ^ 1, gave_up));
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one()) {
-#pragma unroll
-                    for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8(tmem + b * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0);
-                    tc_commit(done + 8 * b);
-                    tc_commit(empty + 8 * s);
-                }
-            }
-        }
-        if (!ok && elect_one()) {  // the instructions in flight end before their memory is given back
-            tc_commit(drained);
-            const uint64_t t0 = global_ns();
-            while (!bar_try(drained, 0) && global_ns() - t0 < kDrainLimitNs) {
-            }
-        }
-    } else if (warp == S::kScaling) {  // ---- scales of kAhead column blocks into the next slot, by asynchronous copies
-        RingAt<S::kSlots> at_slot;
-        bool ok = true;
-        while (ok && next_tile()) {
-            const int row = tile.y + lane;
-            const float* const sx = p.x.scales + row * p.x.srs;
-            for (int kb = kb0; kb < kb1; kb += S::kAhead, at_slot.next()) {
-                const uint32_t slot = at_slot.i, at = smem_addr(scales) + slot * S::kSlotBytes;
-                ok = __all_sync(0xffffffffu, bar_wait(slot_read + 8 * slot, at_slot.phase ^ 1, gave_up));
-                if (!ok) break;
-#pragma unroll
-                for (int a = 0; a < S::kAhead; ++a)
-#pragma unroll
-                    for (int i = 0; i < (S::kTileRows + 31) / 32; ++i) {
-                        if (S::kTileRows < 32 && lane >= S::kTileRows) break;
-                        const bool in = kb + a < kb1 && row + 32 * i < tile.z;
-                        copy_word_async(at + (a * S::kTileRows + 32 * i + lane) * 4, in ? sx + 32 * i * p.x.srs + (kb + a) * p.x.scs : p.x.scales, in);
+                if (!more) break;
+                for (int kb = kb0; kb < kb1; ++kb, ++it, at_stage.next()) {
+                    const uint32_t s = at_stage.i, at = smem_addr(ring) + s * S::kStageBytes;
+                    ok = __all_sync(0xffffffffu, bar_wait(empty + 8 * s, at_stage.phase ^ 1, gave_up));
+                    if (!ok) break;
+                    if (elect_one()) {
+                        bar_expect(full + 8 * s, S::kStageBytes);
+                        tma_load_3d(S::SWAP ? at : at + 128 * kBlock, &wmap, full + 8 * s, kb * kBlock, walk.n_tile * S::kOutputs, walk.expert);
+                        tma_load_2d(S::SWAP ? at + 128 * kBlock : at, &xmap, full + 8 * s, kb * kBlock, walk.row0);
                     }
-                if (lane < S::kTileBlocks * S::kAhead) {
-                    const int a = lane % S::kAhead;
-                    const bool in = kb + a < kb1;
-                    const int64_t wb = min((int64_t(tile.w) * S::kOutputs + (S::SWAP ? 0 : lane / S::kAhead * S::kCols)) / 128, p.w.row_blocks - 1);
-                    copy_word_async(at + (S::kAhead * S::kTileRows + lane) * 4, in ? p.w.scales + tile.x * p.w.sms + wb * p.w.srs + (kb + a) * p.w.scs : p.w.scales, in);
                 }
-                bar_arrive_copies(slot_full + 8 * slot);
             }
+            if (ok && lane == 0)  // every arrival at the ring's barriers has happened before the CTA ends
+                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) bar_wait(empty + 8 * (i % STAGES), (i / STAGES) & 1, gave_up);
+            if (!ok && lane == 0)  // the copies in flight land before the CTA ends
+                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
+                    const uint64_t t0 = global_ns();
+                    while (!bar_try(full + 8 * (i % STAGES), (i / STAGES) & 1) && global_ns() - t0 < kDrainLimitNs) {
+                    }
+                }
+        } else if (warp == S::kIssue) {  // ---- matrix instructions
+            RingAt<STAGES> at_stage;
+            RingAt<NBUF> at_sum;
+            bool ok = true;
+            while (ok && next_tile()) {
+                for (int kb = kb0; kb < kb1; ++kb, at_stage.next(), at_sum.next()) {
+                    const uint32_t s = at_stage.i, b = at_sum.i;
+                    const uint32_t at = smem_addr(ring) + s * S::kStageBytes;
+                    const uint64_t ad = tc_operand(at), bd = tc_operand(at + 128 * kBlock);
+                    // the accumulator last: with it the time between two uses of one accumulator starts to run
+                    ok = __all_sync(0xffffffffu, bar_wait(full + 8 * s, at_stage.phase, gave_up) && bar_wait(taken + 8 * b, at_sum.phase ^ 1, gave_up));
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < kBlock / 32; ++k) tc_mma_f8(tmem + b * BN, ad + 2 * k, bd + 2 * k, idesc, k > 0);
+                        tc_commit(done + 8 * b);
+                        tc_commit(empty + 8 * s);
+                    }
+                }
+            }
+            if (!ok && elect_one()) {  // the instructions in flight end before their memory is given back
+                tc_commit(drained);
+                const uint64_t t0 = global_ns();
+                while (!bar_try(drained, 0) && global_ns() - t0 < kDrainLimitNs) {
+                }
+            }
+        } else if (warp == S::kScaling) {  // ---- scales of kAhead column blocks into the next slot, by asynchronous copies
+            RingAt<S::kSlots> at_slot;
+            bool ok = true;
+            while (ok && next_tile()) {
+                const int row = tile.y + lane;
+                const float* const sx = p.x.scales + row * p.x.srs;
+                for (int kb = kb0; kb < kb1; kb += S::kAhead, at_slot.next()) {
+                    const uint32_t slot = at_slot.i, at = smem_addr(scales) + slot * S::kSlotBytes;
+                    ok = __all_sync(0xffffffffu, bar_wait(slot_read + 8 * slot, at_slot.phase ^ 1, gave_up));
+                    if (!ok) break;
+#pragma unroll
+                    for (int a = 0; a < S::kAhead; ++a)
+#pragma unroll
+                        for (int i = 0; i < (S::kTileRows + 31) / 32; ++i) {
+                            if (S::kTileRows < 32 && lane >= S::kTileRows) break;
+                            const bool in = kb + a < kb1 && row + 32 * i < tile.z;
+                            copy_word_async(at + (a * S::kTileRows + 32 * i + lane) * 4, in ? sx + 32 * i * p.x.srs + (kb + a) * p.x.scs : p.x.scales, in);
+                        }
+                    if (lane < S::kTileBlocks * S::kAhead) {
+                        const int a = lane % S::kAhead;
+                        const bool in = kb + a < kb1;
+                        const int64_t wb = min((int64_t(tile.w) * S::kOutputs + (S::SWAP ? 0 : lane / S::kAhead * S::kCols)) / 128, p.w.row_blocks - 1);
+                        copy_word_async(at + (S::kAhead * S::kTileRows + lane) * 4, in ? p.w.scales + tile.x * p.w.sms + wb * p.w.srs + (kb + a) * p.w.scs : p.w.scales, in);
+                    }
+                    bar_arrive_copies(slot_full + 8 * slot);
+                }
+            }
+            copies_wait_all();
         }
-        copies_wait_all();
-    }
     } else {  // ---- epilogue
         if constexpr (S::kTrades) regs_take<kTaken>();
         constexpr int kCols = S::kCols;
@@ -359,47 +371,47 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
             for (int i = 0; i < kCols / 2; ++i) acc[i] = 0;
             const float* const my_scale = scales + (S::SWAP ? col0 : quarter * 32 + lane);
             const float* const my_weight = scales + S::kAhead * S::kTileRows + (S::SWAP ? 0 : warp / 4 * S::kAhead);
-            // The waits' results are looked at once per tile: a warp that only goes on after all of its lanes have agreed
-            // lost 80 cycles per column block.
+            // A wait that gave up is looked at once per tile (a vote after every wait cost 80 cycles per column block): what the warps
+            // read until then is not meant, but lies where it should.
             for (int kb = kb0; kb < kb1; kb += S::kAhead, at_slot.next()) {
-              bar_wait(slot_full + 8 * at_slot.i, at_slot.phase, gave_up);
-              const float* sx = my_scale + at_slot.i * (S::kSlotBytes / 4);
-              const float* sw = my_weight + at_slot.i * (S::kSlotBytes / 4);
-              for (int left = min(S::kAhead, kb1 - kb); left > 0; --left, sx += S::kTileRows, ++sw, at_sum.next()) {
-                const uint32_t b = at_sum.i;
-                float scale = *sw;
-                if (!S::SWAP) scale = __fmul_rn(*sx, scale);
-                const uint64_t s2 = pack2(__float_as_uint(scale), __float_as_uint(scale));
-                bar_wait(done + 8 * b, at_sum.phase, gave_up);
-                __syncwarp();
-                tc_fence_after();
-                uint32_t v[2][S::LOAD];  // one part being multiplied, the next one on its way
-                tmem_load(v[0], my_tmem + b * BN);
+                bar_wait(slot_full + 8 * at_slot.i, at_slot.phase, gave_up);
+                const float* sx = my_scale + at_slot.i * (S::kSlotBytes / 4);
+                const float* sw = my_weight + at_slot.i * (S::kSlotBytes / 4);
+                for (int todo = min(S::kAhead, kb1 - kb); todo > 0; --todo, sx += S::kTileRows, ++sw, at_sum.next()) {
+                    const uint32_t b = at_sum.i;
+                    float scale = *sw;
+                    if (!S::SWAP) scale = __fmul_rn(*sx, scale);
+                    const uint64_t s2 = pack2(__float_as_uint(scale), __float_as_uint(scale));
+                    bar_wait(done + 8 * b, at_sum.phase, gave_up);
+                    __syncwarp();
+                    tc_fence_after();
+                    uint32_t v[2][S::LOAD];  // one part being multiplied, the next one on its way
+                    tmem_load(v[0], my_tmem + b * BN);
 #pragma unroll
-                for (int c = 0; c < kCols; c += S::LOAD) {
-                    uint32_t(&u)[S::LOAD] = v[c / S::LOAD & 1];
-                    tmem_load_wait(u);
-                    if (c + S::LOAD < kCols) tmem_load(v[(c / S::LOAD + 1) & 1], my_tmem + b * BN + c + S::LOAD);
-                    if (c + S::LOAD == kCols) {  // all of it is in registers: the accumulator may be written again
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) bar_arrive(taken + 8 * b);
-                    }
-                    if constexpr (S::SWAP) {
-#pragma unroll
-                        for (int i = 0; i < S::LOAD; i += 4) {
-                            const uint4 s4 = *reinterpret_cast<const uint4*>(sx + c + i);
-                            fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), mul2(pack2(s4.x, s4.y), s2));
-                            fma2(acc[(c + i) / 2 + 1], pack2(u[i + 2], u[i + 3]), mul2(pack2(s4.z, s4.w), s2));
+                    for (int c = 0; c < kCols; c += S::LOAD) {
+                        uint32_t(&u)[S::LOAD] = v[c / S::LOAD & 1];
+                        tmem_load_wait(u);
+                        if (c + S::LOAD < kCols) tmem_load(v[(c / S::LOAD + 1) & 1], my_tmem + b * BN + c + S::LOAD);
+                        if (c + S::LOAD == kCols) {  // all of it is in registers: the accumulator may be written again
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(taken + 8 * b);
                         }
-                    } else {
+                        if constexpr (S::SWAP) {
 #pragma unroll
-                        for (int i = 0; i < S::LOAD; i += 2) fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), s2);
+                            for (int i = 0; i < S::LOAD; i += 4) {
+                                const uint4 s4 = *reinterpret_cast<const uint4*>(sx + c + i);
+                                fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), mul2(pack2(s4.x, s4.y), s2));
+                                fma2(acc[(c + i) / 2 + 1], pack2(u[i + 2], u[i + 3]), mul2(pack2(s4.z, s4.w), s2));
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < S::LOAD; i += 2) fma2(acc[(c + i) / 2], pack2(u[i], u[i + 1]), s2);
+                        }
                     }
                 }
-              }
-              __syncwarp();
-              if (lane == 0) bar_arrive(slot_read + 8 * at_slot.i);
+                __syncwarp();
+                if (lane == 0) bar_arrive(slot_read + 8 * at_slot.i);
             }
             ok = !__any_sync(0xffffffffu, *gave_up);
             if (!ok) break;
