@@ -5,6 +5,7 @@
 // patterns with the sign cleared: for floats their order as integers is the order of the magnitudes, 16-bit types are
 // compared two at a time, and infinities and NaN sort above every number, so the maximum also tells whether there was one.
 #include "block_device.cuh"
+#include "tensor_core.cuh"
 
 namespace vf {
 
@@ -78,6 +79,12 @@ __device__ __forceinline__ float magnitude(uint32_t m) {
     else return __uint_as_float(h << 16);
 }
 
+// two products, each rounded as the single multiplication rounds
+__device__ __forceinline__ float2 times(float2 a, float s) {
+    const uint64_t r = mul2(pack2(__float_as_uint(a.x), __float_as_uint(a.y)), pack2(__float_as_uint(s), __float_as_uint(s)));
+    return make_float2(__uint_as_float(uint32_t(r)), __uint_as_float(uint32_t(r >> 32)));
+}
+
 struct Scale {
     float scale, inverse;
 };
@@ -95,8 +102,10 @@ template <class T, bool E5M2>
 __device__ __forceinline__ uint2 codes_of(const Eight<T>& v, float inverse) {
     uint32_t c[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        c[i] = to_codes<E5M2>(__fmul_rn(value_of<T>(v, 2 * i), inverse), __fmul_rn(value_of<T>(v, 2 * i + 1), inverse));
+    for (int i = 0; i < 4; ++i) {
+        const float2 q = times(make_float2(value_of<T>(v, 2 * i), value_of<T>(v, 2 * i + 1)), inverse);
+        c[i] = to_codes<E5M2>(q.x, q.y);
+    }
     return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
 }
 
@@ -115,8 +124,8 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int n) {
 // 256 columns of Rows rows, whose loads are in flight together. The rows' maxima are found by halves: lanes that differ in
 // bit 3 of their position exchange what the other one keeps, then bit 2, bit 1, so that after Rows - 1 exchanges instead of
 // 4 * Rows a lane is left with one row, for which it alone divides.
-//   [8192, 11008] bf16: 46.0 us with eight rows (5.9 TB/s), 54.9 with four, 60.6 with two; 59 us with four when every lane divided
-//   for every row. [1, 4096]: 2.5 us with eight, 1.6 with two.
+//   [8192, 11008] bf16: 43.9 us with eight rows (6.2 TB/s), 54.9 with four, 60.6 with two; 59 us with four when every lane divided
+//   for every row. [1, 4096]: 2.5 us with eight, 1.6 with two. Bound by memory (issue slots 62 % busy).
 template <class T, int Rows, bool E5M2, bool Aligned>
 __global__ void __launch_bounds__(kThreads, 4) k_quantize_tokens(const T* __restrict__ base, int64_t base_ld, Blocks b, int64_t col_tiles, int64_t tiles,
                                                                  int* flags) {
@@ -172,7 +181,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_quantize_tokens(const T* __rest
 }
 
 // Weight blocks: a CTA owns 128 x 128 elements, eight loads of eight elements per thread, all in flight before the
-// maximum is taken; the elements stay in registers until the codes are written.
+// maximum is taken; the elements stay in registers until the codes are written. [11008, 4096] f16: 26.3 us (5.1 TB/s; [28672, 8192]
+// 118 us, 6.0 TB/s: 2752 tiles make 4.6 rounds). Tried: 512 threads with four loads each 27.7, five CTAs per multiprocessor 28.7 (it
+// spills), a persistent grid 26.9, rows of blocks before columns 28.0.
 template <class T, bool E5M2, bool Aligned>
 __global__ void __launch_bounds__(kThreads) k_quantize_weights(const T* __restrict__ base, int64_t base_ld, Blocks b, int64_t tiles, int* flags) {
     chain_enter();
@@ -214,7 +225,7 @@ __global__ void __launch_bounds__(kThreads) k_quantize_weights(const T* __restri
 
 // Reading back: a lane turns the codes behind one 16-byte store into it (8 codes for a 16-bit type, 4 for f32), so that
 // every store instruction of a warp is one run of 512 bytes; Rows rows are in flight per warp.
-// 11008 x 4096 to f16: 24.5 us with eight, 25.3 with four, 28.3 with two; [1003, 1111] to f32: 4.0 us with eight, 3.2 with two.
+// 11008 x 4096 to f16: 23.7 us with eight, 25.3 with four, 28.3 with two; [1003, 1111] to f32: 4.0 us with eight, 3.2 with two.
 template <class T, int Rows, bool E5M2, bool Aligned>
 __global__ void __launch_bounds__(kThreads, 4) k_dequantize_blocks(Blocks b, T* __restrict__ dst, int64_t dst_ld, int64_t col_tiles, int64_t tiles) {
     chain_enter();
@@ -256,9 +267,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_dequantize_blocks(Blocks b, T* 
             alignas(16) T out[kPer];
 #pragma unroll
             for (int k = 0; k < kPer; k += 2) {
-                const float2 f = from_codes((w[i][k / 4] >> (8 * (k & 3))) & 0xFFFFu, E5M2);
-                out[k] = to_wide<T>(__fmul_rn(f.x, s[i]));
-                out[k + 1] = to_wide<T>(__fmul_rn(f.y, s[i]));
+                const float2 f = times(from_codes((w[i][k / 4] >> (8 * (k & 3))) & 0xFFFFu, E5M2), s[i]);
+                out[k] = to_wide<T>(f.x);
+                out[k + 1] = to_wide<T>(f.y);
             }
             T* q = dst + (r0 + i) * dst_ld + c;
             if (Aligned && n == kPer) {
@@ -313,7 +324,7 @@ void launch_quantize_blocks(vf_ctx* ctx, const void* base, int base_dt, int64_t 
         with_flag(b.dtype == VF_DT_F8E5M2, [&](auto e5) {
             with_flag(al, [&](auto vec) {
                 using T = decltype(t);
-                constexpr int kMany = sizeof(T) == 4 ? 4 : 8;  // (registers)
+                constexpr int kMany = sizeof(T) == 4 || !vec.value ? 4 : 8;  // (registers)
                 const T* src = static_cast<const T*>(base);
                 if (b.block_rows == 1) {
                     const bool small = is_small(ctx, rows * b.cols);
