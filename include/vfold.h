@@ -221,8 +221,8 @@ typedef struct vf_transform {
 typedef struct vf_ctx vf_ctx;
 
 #define VF_OPT_DISABLE_FUSION 1 /* run vf_quantize_fold through the unfused general kernels (for cross-checks) */
-/* Pipelined calls: vf_fold, vf_fold_batch, vf_quantize_fold_batch, vf_weights_table_batch and vf_sparsify_batch
- * calls whose tensors ALL live in device memory return as soon as their work is enqueued on the context's stream,
+/* Pipelined calls: vf_fold, vf_fold_batch, vf_quantize_fold_batch, vf_weights_table_batch, vf_sparsify_batch,
+ * vf_quantize_blocks, vf_dequantize_blocks and vf_matmul_blocks[_grouped] calls whose tensors ALL live in device memory return as soon as their work is enqueued on the context's stream,
  * so the host prepares the next batch while the GPU runs this one (what the background folder does with its
  * thread pool, const/utils/constant_folding_in_background.cpp:154-194). Host-side checks (shapes, types, sizes)
  * still fail the call itself; what a kernel reports (a checked_cast, a range without zero, a table range) is
@@ -427,7 +427,8 @@ int vf_dequantize_blocks(vf_ctx* ctx, const vf_block_matrix* in, void* dst, int3
  * (0 = N). Per 128 columns the codes are multiplied and summed in fp32, the sum is scaled by the product of the two scales
  * and added in fp32; y is rounded once, to nearest even, overflow to infinity. Everything lives in DEVICE memory;
  * M = 0 or N = 0 writes nothing. Operands whose codes start on 16-byte boundaries with `ld` (and matrix_stride) a
- * multiple of 16 run on the tensor cores, others on a plain kernel that is tens of times slower. */
+ * multiple of 16 run on the tensor cores, others on a plain kernel that is tens of times slower. Rows and columns of
+ * tiles are counted in 32 bits: a claim of 2^30 tiles or more is refused (VF_ERR_CAPACITY). */
 int vf_matmul_blocks(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matrix* w, void* out, int32_t out_dtype,
                      int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err, size_t errlen);
 
@@ -439,6 +440,11 @@ int vf_matmul_blocks(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matri
 int vf_matmul_blocks_grouped(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matrix* w, const int64_t* offsets, void* out,
                              int32_t out_dtype, int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err,
                              size_t errlen);
+
+/* All four enqueue one kernel on the context's stream and, on device memory, use no scratch: with VF_OPT_ASYNC and an
+ * `external_stream` they can be captured into a graph (call each once before, so that its kernels are loaded). The
+ * context has to outlive the graph; what the kernels of a replay find is reported by the next synchronising call that
+ * follows a call of the context. */
 
 /* ------------------------------------------------------------------ */
 /* sparsity                                                            */
