@@ -1,6 +1,7 @@
 """8-bit floating-point blocks on the GPU against their restatement in 64 bits (block_reference.py): quantising and
 reading back bit for bit, products within the error their arithmetic can make, each at the sizes, strides, types and
 group borders where a kernel can go wrong, and a run of them together."""
+import os
 import threading
 
 import numpy as np
@@ -16,6 +17,7 @@ E4M3, E5M2 = abi.VF_DT_F8E4M3FN, abi.VF_DT_F8E5M2
 F32, F16, BF16 = abi.VF_DT_F32, abi.VF_DT_F16, abi.VF_DT_BF16
 DEV, HOST = abi.VF_MEM_DEVICE, abi.VF_MEM_HOST
 GUARD = 0xA5
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
 @pytest.fixture(scope="module")
@@ -384,6 +386,76 @@ def test_elements_beyond_32_bits(gpu, torch):
     gpu.matmul_blocks_grouped(xm.pod, wm, offs.data_ptr(), out.data_ptr(), F32, out.nbytes)
     check_product(out[:, -256:].double().cpu().numpy(), xc, xs, wc, ws, E4M3, E4M3, F32, 5, 12)
     assert (out[:5] == 0).all() and (out[5:, :-256] == 0).all()
+
+
+@pytest.mark.parametrize("n", [1, 200])
+def test_one_row_has_no_pitch(gpu, torch, n):
+    """One token of odd width, dense: its row pitch is not a multiple of 16 and does not have to be."""
+    rng = np.random.default_rng(30)
+    for k in (1, 15, 1001, 4099):
+        ops = operands(rng, 1, n, k, E4M3, E4M3)
+        for w_kw in ({"ld": up16(k)}, {"ld": k}):
+            got = run_product(gpu, torch, *ops, E4M3, E4M3, F32, x_kw={"ld": k}, w_kw=w_kw)
+            check_product(got, *ops, E4M3, E4M3, F32)
+
+
+def test_captured_without_a_call_before(torch, tmp_path):
+    """The first calls of a process, recorded into a graph: nothing about them waits or allocates."""
+    import subprocess
+    import sys
+    script = tmp_path / "first.py"
+    script.write_text(FIRST_CALLS_CAPTURED)
+    r = subprocess.run([sys.executable, str(script)], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.strip().endswith("equal"), r.stdout + r.stderr
+
+
+FIRST_CALLS_CAPTURED = """
+import sys
+sys.path.insert(0, ".")
+import torch
+from vpux_plugin_b200 import abi
+from vpux_plugin_b200.lib import Library
+stream = torch.cuda.Stream()
+lib = Library(device=0, stream=stream.cuda_stream, pipelined=True)
+outs = {}
+keep = []
+for m in (1, 20, 40, 100, 3000):
+    x = torch.randn(m, 512, device="cuda")
+    w = torch.randn(2, 3000, 512, device="cuda")
+    xc, xs = torch.zeros(m, 512, dtype=torch.uint8, device="cuda"), torch.zeros(4, m, device="cuda")
+    wc, ws = torch.zeros(2, 3000, 512, dtype=torch.uint8, device="cuda"), torch.zeros(2, 24, 4, device="cuda")
+    y, yg = torch.zeros(m, 3000, device="cuda"), torch.zeros(m, 3000, device="cuda")
+    off = torch.tensor([0, m // 2, m], device="cuda")
+    xm = abi.block_matrix(xc.data_ptr(), xs.data_ptr(), abi.VF_DT_F8E4M3FN, 1, m, 512, scale_row_stride=1, scale_col_stride=m)
+    wm = abi.block_matrix(wc.data_ptr(), ws.data_ptr(), abi.VF_DT_F8E4M3FN, 128, 3000, 512, count=2)
+    w0 = abi.block_matrix(wc.data_ptr(), ws.data_ptr(), abi.VF_DT_F8E4M3FN, 128, 3000, 512)
+    cx, k1 = abi.make_content(abi.TType([m, 512], abi.VF_DT_F32), None, ptr=x.data_ptr(), nbytes=x.nbytes, mem_kind=abi.VF_MEM_DEVICE)
+    cw, k2 = abi.make_content(abi.TType([2, 3000, 512], abi.VF_DT_F32), None, ptr=w.data_ptr(), nbytes=w.nbytes, mem_kind=abi.VF_MEM_DEVICE)
+
+    def calls():
+        lib.quantize_blocks(cx, xm)
+        lib.quantize_blocks(cw, wm)
+        lib.matmul_blocks(xm, w0, y.data_ptr(), abi.VF_DT_F32, y.nbytes)
+        lib.matmul_blocks_grouped(xm, wm, off.data_ptr(), yg.data_ptr(), abi.VF_DT_F32, yg.nbytes)
+        lib.dequantize_blocks(wm, w.data_ptr(), abi.VF_DT_F32, w.nbytes)
+
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        calls()
+    g.replay()
+    torch.cuda.synchronize()
+    first = (y.clone(), yg.clone(), w.clone())
+    y.zero_(), yg.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        calls()
+    lib.synchronize()
+    for a, b in zip(first, (y, yg, w)):
+        assert float(a.abs().max()) > 1 and torch.equal(a, b), m
+    del g
+print("equal")
+"""
 
 
 def test_a_claim_of_more_tiles_than_fit_is_refused(gpu):

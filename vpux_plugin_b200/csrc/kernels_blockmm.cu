@@ -504,11 +504,17 @@ EncodeTiled encode_tiled() {
     return f;
 }
 
+// A single row has no second one to be a pitch away from.
+int64_t row_pitch(const Blocks& b) {
+    return b.rows == 1 ? align_up(b.cols, 16) : b.ld;
+}
+
 // Boxes of `box_rows` rows by 128 columns of a matrix (rank 2) or a stack of them (rank 3); what lies outside reads as zero.
 CUtensorMap map_codes(const Blocks& b, int rank, int box_rows) {
     CUtensorMap m;
     const cuuint64_t dim[3] = {cuuint64_t(b.cols), cuuint64_t(b.rows), cuuint64_t(b.count)};
-    const cuuint64_t stride[2] = {cuuint64_t(b.ld), cuuint64_t(b.count > 1 ? b.matrix_stride : b.ld)};
+    const int64_t ld = row_pitch(b);
+    const cuuint64_t stride[2] = {cuuint64_t(ld), cuuint64_t(b.count > 1 ? b.matrix_stride : ld)};
     const cuuint32_t box[3] = {kBlock, cuuint32_t(box_rows), 1}, one[3] = {1, 1, 1};
     CUresult r = CUDA_SUCCESS;
     for (int attempt = 0; attempt < 2; ++attempt) {
@@ -524,7 +530,7 @@ CUtensorMap map_codes(const Blocks& b, int rank, int box_rows) {
 }
 
 bool fits_bulk_copies(const Blocks& b) {  // start and pitches of 16-byte units, pitches below 2^40 bytes
-    return (reinterpret_cast<uintptr_t>(b.codes) & 15u) == 0 && b.ld % 16 == 0 && b.ld < (int64_t(1) << 40) &&
+    return (reinterpret_cast<uintptr_t>(b.codes) & 15u) == 0 && row_pitch(b) % 16 == 0 && row_pitch(b) < (int64_t(1) << 40) &&
            (b.count == 1 || (b.matrix_stride % 16 == 0 && b.matrix_stride < (int64_t(1) << 40)));
 }
 
