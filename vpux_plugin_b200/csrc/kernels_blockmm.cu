@@ -104,13 +104,14 @@ void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
 // tiles and copies them in (bulk tensor copies into a ring of STAGES), one that issues the matrix instructions, and one that
 // brings the scales of eight column blocks at a time into a ring of their own.
 //
-// Measured ([rows, outputs, columns], back to back, graph replay): [4096, 11008, 4096] 180 us, 2.05 PFLOP/s, tensor pipe active 53 %
-// of the time; 912 cycles per column block and tile, of which the tensor core needs 512. What bounds it: two
-// accumulators of 256 columns fill the tensor memory, and from one use of an accumulator to the next pass the instructions (512),
-// the epilogue's 480 cycles of reading it and three hand-overs through barriers; and the power limit (1.6 GHz under this load).
-// Tried: pairs of CTAs (256 x 256 tiles) 177-184 us, 128 x 192 tiles 206, four epilogue groups 193-199, four accumulators of 128
-// columns 227-247, 32 columns per load 190, the column-block loop unrolled twice 221-290 (it spills). [1, 11008, 4096] 10.6 us and
-// [48, 4096, 11008] 13.8 us at 4.3 and 3.3 TB/s of weights; [1, 32000, 8192] 43.4 us at 6.0 TB/s: a launch costs 3.5 us of its own.
+// Measured ([rows, outputs, columns], back to back, graph replay): [4096, 11008, 4096] 164 us, 2.26 PFLOP/s; about 820 cycles per
+// column block and tile, of which the tensor core needs 512. What bounds it: two accumulators of 256 columns fill the tensor
+// memory, and from one use of an accumulator to the next pass the instructions (512), the epilogue's 480 cycles of reading it
+// and three hand-overs through barriers; and the power limit (the clock falls to 1.6 GHz under this load).
+// Tried before the issuing warp became uniform, when this size took 180: pairs of CTAs (256 x 256 tiles) 177-184 us, 128 x 192 tiles
+// 206, four epilogue groups 193-199, 32 columns per load 190, the column-block loop unrolled twice 221-290 (it spills).
+// [1, 11008, 4096] 10.1 us and [48, 4096, 11008] 13.9 us at 4.5 and 3.3 TB/s of weights; [1, 32000, 8192] 43.4 us at 6.0 TB/s: a
+// launch costs 3.5 us of its own, and joining the CTAs of a cluster 1 to 3.
 constexpr int kGiven = 72, kTaken = 216;  // registers per thread after the trade: 128 * 72 + 256 * 216 = 384 * 168
 
 template <bool SWAP_, int BN_, int STAGES_, int NBUF_, int GROUPS_, int PER_SM_, int LOAD_ = 32>
@@ -127,7 +128,7 @@ struct Shape {
     static constexpr int kAhead = 8, kSlots = 2, kTileRows = SWAP ? BN : 128, kTileBlocks = SWAP ? 1 : GROUPS;
     static constexpr int kSlotBytes = kAhead * (kTileRows + kTileBlocks) * 4;
     static constexpr int kStageBytes = (128 + BN) * kBlock;
-    static constexpr int kTmem = NBUF * BN <= 64 ? 64 : (NBUF * BN <= 128 ? 128 : (NBUF * BN <= 256 ? 256 : 512));  // a power of two
+    static constexpr int kTmem = NBUF * BN;  // a power of two
     // clusters share a tile's column blocks: four columns of a tile at a time, the CTAs of a cluster own them in turn
     static constexpr int kFours = BN / 4, kParts = BN == 16 ? 8 : (BN == 32 ? 10 : BN / 4);
     static constexpr int kRing = STAGES * kStageBytes;
@@ -590,16 +591,15 @@ void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
 //                    BN, stages, accumulators, epilogue groups of four warps, CTAs per SM, columns per load
 using Swap16 = Shape<true, 16, 5, 4, 1, 2, 16>;
 using Swap32 = Shape<true, 32, 4, 4, 1, 2, 16>;
-using Swap64 = Shape<true, 64, 3, 4, 1, 2, 16>;
 using Swap128 = Shape<true, 128, 4, 2, 2, 1, 16>;
 using Wide128 = Shape<false, 128, 5, 2, 2, 1, 32>;
 using Wide256 = Shape<false, 256, 3, 2, 2, 1, 16>;
 
 // Few rows: CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column
 // blocks that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs
-// about as much as four of them. (48 rows, 4096 x 11008, 32 tiles of 86 blocks: 40 us alone, 18.7 with four, 13.7 with eight, although
-// the last of 32 such clusters has to wait for a place. Clusters of eight CTAs with a multiprocessor each wait more
-// often: [256, 1024, 8192] in 19.6 us with eight, 15.5 with four.)
+// about as much as four of them. (With tiles of 64 columns, [48, 4096, 11008], 32 tiles of 86 blocks: 40 us alone, 18.7 with four, 13.7
+// with eight, although the last of 32 such clusters has to wait for a place. Clusters of eight CTAs with a multiprocessor each
+// wait more often: [256, 1024, 8192] in 19.6 us with eight, 15.5 with four.)
 template <class S, class T>
 void launch_swapped(vf_ctx* ctx, const BlockProduct& p) {
     const int64_t tiles = most_tiles(p, S::BN, 128);
@@ -615,28 +615,33 @@ void launch_swapped(vf_ctx* ctx, const BlockProduct& p) {
     launch_tensor<S, T>(ctx, p, best);
 }
 
-// The form goes by the rows of activations (of an expert, on average). Times in us, [rows, outputs, columns]:
-//   up to 16      [16, 4096, 4096]    Swap16 6.7   Swap32 7.0   Swap64 8.5
-//   up to 32      [32, 11008, 4096]   Swap16 15.8  Swap32 12.2  Swap64 15.7
-//   up to 64      [33, 11008, 4096]   Swap32 17.2  Swap64 15.9  Swap128 18.6; grouped, 57 rows on average, 16 experts [2048, 2048]:
-//                 Swap32 19.9  Swap64 26.1  Swap128 23.5, since most experts' rows end inside a tile
-//   above, where tiles of 128 x 128 leave half of the multiprocessors idle, Swap128 splits them:
-//                 [128, 4096, 4096]   Swap128 10.9  Wide128 15.3  Wide256 17.6; [192, 4096, 4096] (64 tiles) 14.5, 15.6, 17.8
-//   else by the rounds that the tiles take; one of Wide256's takes 1.2 times as long as one of Wide128's:
-//                 [512, 4096, 4096]   128 or 64 tiles, one round either way: Wide128 16.2  Wide256 18.8
-//                 [1024, 4096, 4096]  256 or 128 tiles, two rounds or one: Wide128 29.1  Wide256 20.5
+// The form goes by the rows of activations (of an expert, on average) and by the tiles that there are. Times in us, [rows, outputs, columns]:
+//   up to 16 rows       [16, 4096, 4096]     Swap16 6.5   Swap32 6.9   Swap128 9.4
+//   up to 32            [32, 11008, 4096]    Swap16 13.7  Swap32 11.7  Swap128 19.4; grouped, 32 rows on average, 16 experts [2048, 2048]:
+//                                            Swap32 19.4  Wide128 17.0  Wide256 16.8, since most experts' rows end inside a tile
+//   up to 64, where tiles of 128 x 128 leave half of the multiprocessors idle:
+//                       [64, 4096, 4096]     Swap32 8.3   Swap128 9.6  ([65, 4096, 4096] Wide128 10.8); else
+//                       [64, 11008, 4096]    Swap32 16.4  Swap128 19.9 ([65, 11008, 4096] Wide128 13.1)
+//   above, where they leave three quarters idle:
+//                       [512, 1024, 8192]    Swap128 14.7  Wide128 18.6  Wide256 26.2; else
+//                       [192, 4096, 4096]    Swap128 14.9  Wide128 11.1  Wide256 15.5
+//   and the rest by the rounds that the tiles take; one of Wide256's takes 1.65 times as long as one of Wide128's:
+//                       [512, 4096, 4096]    128 or 64 tiles, one round either way   Wide128 11.8  Wide256 16.7
+//                       [1024, 4096, 4096]   256 or 128 tiles, two rounds or one     Wide128 20.7  Wide256 18.6
+//                       [1500, 4096, 4096]   three rounds or two                     Wide128 29.8  Wide256 31.8
+//                       [4096, 11008, 4096]  nineteen or ten                         Wide128 191.9 Wide256 163.7
 template <class T>
 void launch_for(vf_ctx* ctx, const BlockProduct& p) {
     if (!fits_bulk_copies(p.x) || !fits_bulk_copies(p.w)) return launch_plain<T>(ctx, p);
-    const int64_t rows = p.offsets ? (p.x.rows + p.w.count - 1) / p.w.count : p.x.rows;
-    if (rows <= 16) return launch_swapped<Swap16, T>(ctx, p);
-    if (rows <= 32 || (p.offsets && rows <= 64)) return launch_swapped<Swap32, T>(ctx, p);
-    if (rows <= 64) return launch_swapped<Swap64, T>(ctx, p);
+    const int64_t rows = p.offsets ? (p.x.rows + p.w.count - 1) / p.w.count : p.x.rows, sms = ctx->sm_count;
     // (of the experts' last tiles, half are counted: the bound that the grid is sized by counts one for every expert)
-    const int64_t row_tiles = (p.x.rows + 127) / 128 + (p.offsets ? p.w.count / 2 : 0), sms = ctx->sm_count;
+    const int64_t row_tiles = (p.x.rows + 127) / 128 + (p.offsets ? p.w.count / 2 : 0);
     const int64_t few = row_tiles * ((p.w.rows + 127) / 128), wide = row_tiles * ((p.w.rows + 255) / 256);
-    if (few * 2 <= sms) return launch_swapped<Swap128, T>(ctx, p);
-    if ((wide + sms - 1) / sms * 12 < (few + sms - 1) / sms * 10) return launch_tensor<Wide256, T>(ctx, p);
+    if (rows <= 16) return launch_swapped<Swap16, T>(ctx, p);
+    if (rows <= 32 && !p.offsets) return launch_swapped<Swap32, T>(ctx, p);
+    if (rows <= 64 && few * 2 <= sms) return launch_swapped<Swap32, T>(ctx, p);
+    if (few * 4 <= sms) return launch_swapped<Swap128, T>(ctx, p);
+    if ((wide + sms - 1) / sms * 165 < (few + sms - 1) / sms * 100) return launch_tensor<Wide256, T>(ctx, p);
     launch_tensor<Wide128, T>(ctx, p);
 }
 
