@@ -442,8 +442,8 @@ int vf_matmul_blocks_grouped(vf_ctx* ctx, const vf_block_matrix* x, const vf_blo
                              size_t errlen);
 
 /* All four enqueue one kernel on the context's stream and, on device memory, use no scratch: with VF_OPT_ASYNC and an
- * `external_stream` they can be captured into a graph. The context has to outlive the graph; what the kernels of a replay find is reported by the next synchronising call that
- * follows a call of the context. */
+ * `external_stream` they can be captured into a graph. The context has to outlive the graph; what the kernels of a
+ * replay find is reported by the next synchronising call that follows a call of the context. */
 
 /* ------------------------------------------------------------------ */
 /* sparsity                                                            */

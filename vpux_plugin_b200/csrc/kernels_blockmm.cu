@@ -104,7 +104,7 @@ void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
 // tiles and copies them in (bulk tensor copies into a ring of STAGES), one that issues the matrix instructions, and one that
 // brings the scales of eight column blocks at a time into a ring of their own.
 //
-// Measured ([rows, outputs, columns], back to back, graph replay): [4096, 11008, 4096] 164 us, 2.26 PFLOP/s; about 820 cycles per
+// Measured ([rows, outputs, columns], back to back, graph replay): [4096, 11008, 4096] 161-164 us, 2.3 PFLOP/s, tensor pipe active 64 % of the time; about 820 cycles per
 // column block and tile, of which the tensor core needs 512. What bounds it: two accumulators of 256 columns fill the tensor
 // memory, and from one use of an accumulator to the next pass the instructions (512), the epilogue's 480 cycles of reading it
 // and three hand-overs through barriers; and the power limit (the clock falls to 1.6 GHz under this load).
