@@ -159,10 +159,15 @@ def prepare(case, seed):
 # ---- the library's operators -------------------------------------------------------------------------------------------
 
 @functools.lru_cache(maxsize=None)
-def _library():
+def _context(device, stream):
     from vpux_plugin_b200.lib import Library
-    stream = torch.cuda.current_stream().cuda_stream or 1  # 1 is the handle of the legacy default stream
-    return Library(device=torch.cuda.current_device(), stream=stream, pipelined=True)
+    return Library(device=device, stream=stream or 1, pipelined=True)  # 1 is the handle of the legacy default stream
+
+
+def _library(device):
+    """The context of torch's current stream on `device`: its calls line up with what torch enqueues there. (The handle is
+    asked for as compiled graphs do it; the stream object of torch.cuda.current_stream() costs as much as a small call.)"""
+    return _context(device, torch._C._cuda_getCurrentRawStream(device))
 
 
 def _matrix(codes, scales, cols, rows, code):
@@ -175,9 +180,10 @@ def _matrix(codes, scales, cols, rows, code):
 
 
 def _handles(s):
-    """What a program keeps next to its buffers: the descriptors of its matrices and the context it calls."""
+    """What a program keeps next to its buffers: the descriptors of its matrices. The context that it calls is made here too."""
     from vpux_plugin_b200 import abi
-    s["lib"] = _library()
+    s["device"] = torch.cuda.current_device()
+    _library(s["device"])
     dt = {"f32": abi.VF_DT_F32, "f16": abi.VF_DT_F16, "bf16": abi.VF_DT_BF16}
     if s["op"] in ("quantize", "dequantize"):
         s["matrix"] = _matrix(s["codes"], s["scales"], s["cols"], s["block_rows"], s["code"])
@@ -192,7 +198,7 @@ def _handles(s):
 
 
 def _own(s):
-    lib = s["lib"]
+    lib = _library(s["device"])
     if s["op"] == "quantize":
         lib.quantize_blocks(s["content"], s["matrix"])
         return {"codes": s["codes"].view(CODE[s["code"]])[:, :s["cols"]], "scales": s["scales"]}
