@@ -436,7 +436,8 @@ int vf_matmul_blocks(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matri
  * multiplied by matrix e into the same rows of `out`. `offsets` [w->count + 1] lies in DEVICE memory, starts at 0 or
  * later, does not decrease and ends at or before x->rows; an expert may have no rows. Rows outside
  * offsets[0] .. offsets[count] are left as they are. Offsets that break these rules give VF_ERR_RANGE after the
- * kernel ran; they are clamped to them, so nothing outside the operands is touched. */
+ * kernel ran: they are moved into 0 .. x->rows and up to where the rows of the experts before end, so that nothing outside the
+ * operands is touched and no row is written twice. Without rows or columns no kernel runs and nothing looks at them. */
 int vf_matmul_blocks_grouped(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matrix* w, const int64_t* offsets, void* out,
                              int32_t out_dtype, int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err,
                              size_t errlen);

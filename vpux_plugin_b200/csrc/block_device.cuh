@@ -5,6 +5,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "block_plan.h"
 #include "blocks.h"
 #include "device_utils.cuh"
 
@@ -56,8 +57,8 @@ __device__ __forceinline__ __nv_bfloat16 to_wide<__nv_bfloat16>(float v) {
 // Walks the tiles of a product in ascending order. A tile is `bm` rows of one expert by one of `n_tiles` column tiles;
 // the tiles of expert e come before those of e + 1, and within an expert the row tiles of a column tile follow one
 // another, so that tiles which run at the same time share the weights. Without offsets all rows form one group. Every method is
-// called by whole warps; the number of tiles fits 32 bits (most_tiles() sees to it). Offsets are read 32 at a time, one expert per lane; they are clamped into the operand, and
-// offsets that had to be clamped set a flag.
+// called by whole warps; the number of tiles fits 32 bits (most_tiles() sees to it). Offsets are read 32 at a time, one expert
+// per lane. Offsets that break the rules are moved as rows_of() says and set a flag; those that keep them cost one vote.
 struct TileWalk {
     const int64_t* offsets;
     int* flags;
@@ -67,24 +68,40 @@ struct TileWalk {
     int base;              // tiles before expert e0
     int through;           // tiles of experts e0 .. e0 + lane
     int lo, hi;            // this lane's rows
+    int reach;             // where the ranges before expert e0 end
     // the tile found
     int expert, row0, row_end, n_tile;
 
     __device__ __forceinline__ void load() {
-        const int e = e0 + int(threadIdx.x & 31);
-        lo = hi = 0;
-        if (e < experts) {
-            const int64_t a = offsets[e], b = offsets[e + 1];
-            const int64_t ca = a < 0 ? 0 : (a > rows ? rows : a), cb = b < ca ? ca : (b > rows ? rows : b);
-            if (a != ca || b != cb) set_flag(flags, VF_FLAG_OFFSETS);
-            lo = int(ca);
-            hi = int(cb);
+        const int lane = int(threadIdx.x & 31), e = e0 + lane;
+        const bool in = e < experts;
+        const int64_t a = in ? offsets[e] : 0, b = in ? offsets[e + 1] : 0;
+        lo = int(a);
+        hi = int(b);
+        int before = __shfl_up_sync(0xffffffffu, hi, 1);
+        if (lane == 0) before = reach;
+        if (__all_sync(0xffffffffu, !in || (a >= 0 && a <= b && b <= rows && lo >= before))) {
+            reach = __shfl_sync(0xffffffffu, hi, 31);  // (looked at only if there are experts behind these)
+        } else {
+            int to = max(reach, in ? row_reach(a, b, rows) : 0);
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int o = __shfl_up_sync(0xffffffffu, to, d);
+                if (lane >= d) to = max(to, o);
+            }
+            before = __shfl_up_sync(0xffffffffu, to, 1);
+            if (lane == 0) before = reach;
+            const RowRange r = rows_of(a, b, rows, before);
+            if (in && r.moved) set_flag(flags, VF_FLAG_OFFSETS);
+            lo = in ? r.lo : 0;
+            hi = in ? r.hi : 0;
+            reach = __shfl_sync(0xffffffffu, to, 31);
         }
-        through = int(uint32_t(hi - lo + bm - 1) / uint32_t(bm)) * n_tiles;
+        through = tiles_of_rows(lo, hi, bm) * n_tiles;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const int o = __shfl_up_sync(0xffffffffu, through, d);
-            if (int(threadIdx.x & 31) >= d) through += o;
+            if (lane >= d) through += o;
         }
     }
     __device__ __forceinline__ void start(const int64_t* offs, int n_experts, int64_t n_rows, int tile_rows, int col_tiles, int* err_flags) {
@@ -96,6 +113,7 @@ struct TileWalk {
         flags = err_flags;
         e0 = 0;
         base = 0;
+        reach = 0;
         if (offsets) load();
     }
     // Finds tile `t` (not below the one found before); false behind the last tile.
@@ -125,7 +143,7 @@ struct TileWalk {
         const int src = __ffs(__ballot_sync(0xffffffffu, through > rel)) - 1;
         const int l = __shfl_sync(0xffffffffu, lo, src), h = __shfl_sync(0xffffffffu, hi, src);
         const int before = __shfl_sync(0xffffffffu, through, src ? src - 1 : 0);
-        const int m_tiles = int(uint32_t(h - l + bm - 1) / uint32_t(bm));
+        const int m_tiles = tiles_of_rows(l, h, bm);
         const int in_expert = src ? rel - before : rel;
         n_tile = int(uint32_t(in_expert) / uint32_t(m_tiles));
         expert = e0 + src;

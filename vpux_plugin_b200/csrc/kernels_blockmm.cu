@@ -65,16 +65,10 @@ __global__ void __launch_bounds__(256) k_matmul_blocks_plain(BlockProduct p, int
     }
 }
 
-// Row tiles of `bm` rows: exact without offsets; with them an upper bound (every expert may end inside a tile).
-int64_t most_row_tiles(const BlockProduct& p, int bm) {
-    const int64_t whole = (p.x.rows + bm - 1) / bm;
-    return p.offsets ? std::min(p.x.rows, whole + p.w.count) : whole;
-}
-
 // Tiles of bm rows by bn columns, as an upper bound. The kernels count them (and one step of their grid) in 32 bits: a result
 // with so many tiles does not fit the device's memory, a claim of one is refused.
 int64_t most_tiles(const BlockProduct& p, int bm, int bn) {
-    const int64_t rows = most_row_tiles(p, bm), cols = (p.w.rows + bn - 1) / bn;
+    const int64_t rows = most_row_tiles(p.x.rows, p.offsets ? p.w.count : 0, bm), cols = (p.w.rows + bn - 1) / bn;
     if (rows > (int64_t(1) << 30) / cols) raise(VF_ERR_CAPACITY, "a product of %lld by %lld tiles", (long long)rows, (long long)cols);
     return rows * cols;
 }
@@ -277,7 +271,11 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
             RingAt<STAGES> at_stage;
             bool ok = true;
             for (int t = blockIdx.x / ranks; ok; t += gridDim.x / ranks, ++turn) {
-                const bool more = walk.find(t);
+                bool more = walk.find(t);
+                if (in_cluster && turn && more) {  // a cluster joins its sums once; the launch has one for every tile that there can be
+                    set_flag(flags, VF_FLAG_OFFSETS);
+                    more = false;
+                }
                 const uint32_t i = turn & 1;
                 ok = __all_sync(0xffffffffu, bar_wait(tile_read + 8 * i, ((turn >> 1) & 1) ^ 1, gave_up));
                 if (!ok) break;
@@ -433,7 +431,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
             T* const out = static_cast<T*>(p.out) + int64_t(tile.y) * p.out_ld + n;
             if (S::SWAP && ranks > 1) {
                 // Four columns go to the CTA that owns them, which has a place for every rank's; the only tile of this
-                // cluster, so nobody has to be asked whether a place is free.
+                // cluster (the copying warp sees to it), so nobody has to be asked whether a place is free.
                 if constexpr (S::SWAP) {
                     const int fours = (min(here, BN) + 3) / 4, mine = fours > int(rank) ? (fours - int(rank) - 1) / int(ranks) + 1 : 0;
                     const int places = (S::kFours + int(ranks) - 1) / int(ranks);
