@@ -130,13 +130,13 @@ BlockProduct checked_product(const vf_block_matrix* x, const vf_block_matrix* w,
     p.out = out;
     p.out_dt = out_dtype;
     p.out_ld = out_ld;
-    const uint64_t span = p.w.rows ? wide_span(out, out_dtype, p.x.rows, p.w.rows, p.out_ld, out_bytes, VF_MEM_DEVICE, "out") : 0;
+    p.out_span = p.w.rows ? wide_span(out, out_dtype, p.x.rows, p.w.rows, p.out_ld, out_bytes, VF_MEM_DEVICE, "out") : 0;
     if (!p.w.rows && !is_wide(out_dtype)) raise(VF_ERR_UNSUPPORTED, "out: f32, f16 or bf16 elements, not type %d", out_dtype);
     const char* what = "the result and an operand";
-    check_apart(out, span, p.x.codes, p.x.codes_span, what);
-    check_apart(out, span, p.x.scales, p.x.scales_span, what);
-    check_apart(out, span, p.w.codes, p.w.codes_span, what);
-    check_apart(out, span, p.w.scales, p.w.scales_span, what);
+    check_apart(out, p.out_span, p.x.codes, p.x.codes_span, what);
+    check_apart(out, p.out_span, p.x.scales, p.x.scales_span, what);
+    check_apart(out, p.out_span, p.w.codes, p.w.codes_span, what);
+    check_apart(out, p.out_span, p.w.scales, p.w.scales_span, what);
     return p;
 }
 
@@ -262,6 +262,7 @@ int vf_matmul_blocks_grouped(vf_ctx* ctx, const vf_block_matrix* x, const vf_blo
         BlockProduct p = checked_product(x, w, out, out_dtype, out_ld, out_bytes);
         if (!offsets) raise(VF_ERR_INVALID_ARG, "offsets is NULL");
         if (reinterpret_cast<uintptr_t>(offsets) & 7u) raise(VF_ERR_ALIGNMENT, "offsets are not 8-byte aligned");
+        check_apart(out, p.out_span, offsets, uint64_t(p.w.count + 1) * 8, "the result and the offsets");
         p.offsets = offsets;
         run_product(ctx, p, stats);
     });

@@ -30,6 +30,7 @@ struct BlockProduct {  // out[m][n] = sum_k x[m][k] w[n][k]; with `offsets`, mat
     void* out = nullptr;
     int out_dt = VF_DT_INVALID;
     int64_t out_ld = 0;
+    uint64_t out_span = 0;  // bytes from the first result to behind the last one
 };
 void launch_matmul_blocks(vf_ctx* ctx, const BlockProduct& p);
 
