@@ -427,8 +427,9 @@ int vf_dequantize_blocks(vf_ctx* ctx, const vf_block_matrix* in, void* dst, int3
  * (0 = N). Per 128 columns the codes are multiplied and summed in fp32, the sum is scaled by the product of the two scales
  * and added in fp32; y is rounded once, to nearest even, overflow to infinity. Everything lives in DEVICE memory;
  * M = 0 or N = 0 writes nothing. Operands whose codes start on 16-byte boundaries with `ld` (and matrix_stride) a
- * multiple of 16 run on the tensor cores, others on a plain kernel that is tens of times slower. Rows and columns of
- * tiles are counted in 32 bits: a claim of 2^30 tiles or more is refused (VF_ERR_CAPACITY). */
+ * multiple of 16 run on the tensor cores, others on a plain kernel that is tens of times slower. Tiles are counted in 32
+ * bits: a claim of more than 2^31 - 2^20 tiles of 16 rows by 64 columns, more than the device's memory holds, is refused
+ * (VF_ERR_CAPACITY). */
 int vf_matmul_blocks(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matrix* w, void* out, int32_t out_dtype,
                      int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err, size_t errlen);
 

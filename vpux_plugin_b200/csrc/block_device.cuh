@@ -57,7 +57,7 @@ __device__ __forceinline__ __nv_bfloat16 to_wide<__nv_bfloat16>(float v) {
 // Walks the tiles of a product in ascending order. A tile is `bm` rows of one expert by one of `n_tiles` column tiles;
 // the tiles of expert e come before those of e + 1, and within an expert the row tiles of a column tile follow one
 // another, so that tiles which run at the same time share the weights. Without offsets all rows form one group. Every method is
-// called by whole warps; the number of tiles fits 32 bits (most_tiles() sees to it). Offsets are read 32 at a time, one expert
+// called by whole warps; the number of tiles fits 32 bits (too_many_tiles() sees to it). Offsets are read 32 at a time, one expert
 // per lane. Offsets that break the rules are moved as rows_of() says and set a flag; those that keep them cost one vote.
 struct TileWalk {
     const int64_t* offsets;

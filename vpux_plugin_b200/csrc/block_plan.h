@@ -49,4 +49,13 @@ inline int64_t most_row_tiles(int64_t rows, int64_t experts, int bm) {
     return experts ? std::min(rows, whole + experts) : whole;
 }
 
+// Tiles are counted in 32 bits, and so is one step of the grid (at most a few thousand) behind the last of them. Whichever form runs,
+// its tiles are not smaller than 16 rows by 64 columns, so a product below this limit by those is counted right by all.
+constexpr int64_t kTileLimit = (int64_t(1) << 31) - (int64_t(1) << 20);
+
+inline bool too_many_tiles(int64_t rows, int64_t experts, int64_t outputs) {
+    const int64_t cols = (outputs + 63) / 64;
+    return cols && most_row_tiles(rows, experts, 16) > kTileLimit / cols;
+}
+
 }  // namespace vf

@@ -2,6 +2,7 @@
 // hold (and are tested) without a device.
 #include <algorithm>
 
+#include "block_plan.h"
 #include "blocks.h"
 #include "call_scope.h"
 
@@ -119,7 +120,7 @@ struct Staged {
     }
 };
 
-BlockProduct checked_product(const vf_block_matrix* x, const vf_block_matrix* w, void* out, int32_t out_dtype, int64_t out_ld, uint64_t out_bytes) {
+BlockProduct checked_product(const vf_block_matrix* x, const vf_block_matrix* w, bool grouped, void* out, int32_t out_dtype, int64_t out_ld, uint64_t out_bytes) {
     BlockProduct p;
     p.x = checked(x, "x");
     p.w = checked(w, "w");
@@ -127,6 +128,9 @@ BlockProduct checked_product(const vf_block_matrix* x, const vf_block_matrix* w,
     if (p.x.block_rows != 1 || p.w.block_rows != kBlock) raise(VF_ERR_UNSUPPORTED, "a product multiplies activations (block_rows 1) by weights (block_rows %d)", kBlock);
     if (p.x.count != 1) raise(VF_ERR_SHAPE, "x is one matrix, not %lld", (long long)p.x.count);
     if (p.x.cols != p.w.cols) raise(VF_ERR_SHAPE, "x has %lld columns, w %lld", (long long)p.x.cols, (long long)p.w.cols);
+    const int64_t experts = grouped ? p.w.count : 0;
+    if (too_many_tiles(p.x.rows, experts, p.w.rows))
+        raise(VF_ERR_CAPACITY, "a product of %lld rows, %lld experts and %lld columns has too many tiles", (long long)p.x.rows, (long long)experts, (long long)p.w.rows);
     p.out = out;
     p.out_dt = out_dtype;
     p.out_ld = out_ld;
@@ -249,7 +253,7 @@ int vf_dequantize_blocks(vf_ctx* ctx, const vf_block_matrix* in, void* dst, int3
 int vf_matmul_blocks(vf_ctx* ctx, const vf_block_matrix* x, const vf_block_matrix* w, void* out, int32_t out_dtype,
                      int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err, size_t errlen) {
     return guard(err, errlen, [&] {
-        const BlockProduct p = checked_product(x, w, out, out_dtype, out_ld, out_bytes);
+        const BlockProduct p = checked_product(x, w, false, out, out_dtype, out_ld, out_bytes);
         if (p.w.count != 1) raise(VF_ERR_SHAPE, "w is one matrix, not %lld (vf_matmul_blocks_grouped takes a stack)", (long long)p.w.count);
         run_product(ctx, p, stats);
     });
@@ -259,7 +263,7 @@ int vf_matmul_blocks_grouped(vf_ctx* ctx, const vf_block_matrix* x, const vf_blo
                              int32_t out_dtype, int64_t out_ld, uint64_t out_bytes, vf_stats* stats, char* err,
                              size_t errlen) {
     return guard(err, errlen, [&] {
-        BlockProduct p = checked_product(x, w, out, out_dtype, out_ld, out_bytes);
+        BlockProduct p = checked_product(x, w, true, out, out_dtype, out_ld, out_bytes);
         if (!offsets) raise(VF_ERR_INVALID_ARG, "offsets is NULL");
         if (reinterpret_cast<uintptr_t>(offsets) & 7u) raise(VF_ERR_ALIGNMENT, "offsets are not 8-byte aligned");
         check_apart(out, p.out_span, offsets, uint64_t(p.w.count + 1) * 8, "the result and the offsets");

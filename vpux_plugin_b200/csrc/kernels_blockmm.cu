@@ -65,12 +65,9 @@ __global__ void __launch_bounds__(256) k_matmul_blocks_plain(BlockProduct p, int
     }
 }
 
-// Tiles of bm rows by bn columns, as an upper bound. The kernels count them (and one step of their grid) in 32 bits: a result
-// with so many tiles does not fit the device's memory, a claim of one is refused.
+// Tiles of bm rows by bn columns, as an upper bound (below kTileLimit: the entry points have refused what is not)
 int64_t most_tiles(const BlockProduct& p, int bm, int bn) {
-    const int64_t rows = most_row_tiles(p.x.rows, p.offsets ? p.w.count : 0, bm), cols = (p.w.rows + bn - 1) / bn;
-    if (rows > (int64_t(1) << 30) / cols) raise(VF_ERR_CAPACITY, "a product of %lld by %lld tiles", (long long)rows, (long long)cols);
-    return rows * cols;
+    return most_row_tiles(p.x.rows, p.offsets ? p.w.count : 0, bm) * ((p.w.rows + bn - 1) / bn);
 }
 
 template <class T>
