@@ -17,7 +17,7 @@ struct CallScope {  // per-call bookkeeping: context lock, device, error flags, 
     vf_stats* stats;
     CallScope(vf_ctx* c, vf_stats* s): ctx(check(c)), lock(c->mu), dev(c->device), launches0(c->launches), stats(s) {
         if (stats) std::memset(stats, 0, sizeof(*stats));
-        flags_clear(ctx);
+        flags_begin(ctx);
         if (stats && ctx->time_ev[0]) cudaEventRecord(ctx->time_ev[0], ctx->stream);
     }
     static vf_ctx* check(vf_ctx* c) {
@@ -45,6 +45,7 @@ struct CallScope {  // per-call bookkeeping: context lock, device, error flags, 
         if (finished) return;
         cudaStreamSynchronize(ctx->main_stream);
         if (ctx->lane_stream) cudaStreamSynchronize(ctx->lane_stream);
+        if (ctx->launches != launches0) flags_drop(ctx);
         cudaGetLastError();
     }
 };

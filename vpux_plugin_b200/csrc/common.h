@@ -247,7 +247,7 @@ struct vf_ctx {
     size_t call_scratch_cap[kScratchSlots] = {0, 0};
     int* d_flags = nullptr;  // device error flags (see VF_FLAG_* in device_utils.cuh)
     int* h_flags = nullptr;  // pinned mirror
-    bool flags_dirty = false;  // the device flags may be non-zero (a call found something or ended early)
+    bool flags_open = false;  // a synchronising call is under way whose findings nobody has read
     bool deferred = false;     // VF_OPT_ASYNC: calls have returned whose kernels are still unchecked
     // VF_OPT_ASYNC, vf_sparsify_batch over device memory: the compressed sizes travel to this pinned area behind the
     // kernels; the next synchronising call writes them into the callers' jobs and checks the capacities
@@ -356,9 +356,11 @@ const void* upload_table(vf_ctx* ctx, const void* src, size_t bytes, DBuf& fallb
 // At least `bytes` of device scratch from slot `slot` of the context (see vf_ctx::call_scratch); NULL when the
 // context is not on its main stream (the caller then takes a buffer of its own).
 void* call_scratch(vf_ctx* ctx, int slot, size_t bytes);
-void flags_clear(vf_ctx* ctx);
+void flags_begin(vf_ctx* ctx);  // at the start of a call
 // synchronises the stream and raises if a kernel recorded an error
 void flags_check(vf_ctx* ctx);
+// for a call that ends early behind kernels of its own: forgets what they found (unless deferred work has to report as well)
+void flags_drop(vf_ctx* ctx);
 
 // Device-resident Const::Content
 struct DContent {

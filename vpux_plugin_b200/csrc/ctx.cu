@@ -126,12 +126,20 @@ void* call_scratch(vf_ctx* ctx, int slot, size_t bytes) {
     return ctx->call_scratch[slot];
 }
 
-// The flags are zero unless a call found something or ended early: only then is the next call's clearing real.
-void flags_clear(vf_ctx* ctx) {
-    if (ctx->deferred) return;  // unchecked work is in flight: its flags and job tables stay as they are
+// Device flags hold what has not been reported yet: findings of deferred calls and of replayed graphs stay until flags_check has
+// read them, which sets them back to zero. Nothing is cleared at the start of a call: a graph that recorded the call would
+// erase at every replay what earlier ones have found.
+void flags_begin(vf_ctx* ctx) {
+    if (ctx->deferred) return;  // unchecked work is in flight: its job tables stay as they are
     ctx->table_used = 0;  // a new call: the previous call's job tables are no longer in use
-    if (ctx->flags_dirty) VF_CUDA(cudaMemsetAsync(ctx->d_flags, 0, sizeof(int) * kNumFlags, ctx->stream));
-    ctx->flags_dirty = true;  // until flags_check has seen them all zero
+    ctx->flags_open = true;  // until flags_check has looked at them
+}
+
+void flags_drop(vf_ctx* ctx) {
+    if (ctx->deferred || !ctx->flags_open) return;
+    cudaMemsetAsync(ctx->d_flags, 0, sizeof(int) * kNumFlags, ctx->main_stream);
+    cudaStreamSynchronize(ctx->main_stream);
+    ctx->flags_open = false;
 }
 
 void flags_check(vf_ctx* ctx) {
@@ -157,7 +165,11 @@ void flags_check(vf_ctx* ctx) {
     const int* f = ctx->h_flags;
     bool any = false;
     for (int i = 0; i < kNumFlags; ++i) any |= f[i] != 0;
-    ctx->flags_dirty = any;
+    ctx->flags_open = false;
+    if (any) {  // reported by this call: back to zero before anything else can run
+        cudaMemsetAsync(ctx->d_flags, 0, sizeof(int) * kNumFlags, ctx->stream);
+        cudaStreamSynchronize(ctx->stream);
+    }
     if (too_small)  // (the compaction kernel's overflow flag is the same finding)
         raise(VF_ERR_BUFFER_TOO_SMALL, "compressed weights need %llu bytes, buffer holds %llu", (unsigned long long)too_small->data_written,
               (unsigned long long)too_small->data_bytes);

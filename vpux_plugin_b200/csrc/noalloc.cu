@@ -71,7 +71,7 @@ extern "C" int vf_sparsify_noalloc(vf_ctx* ctx, const void* weights, int32_t dty
         int64_t* d_counts = counts ? counts : reinterpret_cast<int64_t*>(scratch);
         int64_t* d_offsets = reinterpret_cast<int64_t*>(scratch + size_t(kMaxOC) * 8);
 
-        flags_clear(ctx);
+        flags_begin(ctx);
         launch_sparsity_scan(ctx, weights, dtype, oc, work, sparse_value, d_counts, static_cast<uint8_t*>(map), row_bytes);
         uint64_t total_host = 0;
         if (data) {
@@ -84,6 +84,7 @@ extern "C" int vf_sparsify_noalloc(vf_ctx* ctx, const void* weights, int32_t dty
         }
         if (data_written) *data_written = total_host;  // also when the buffer is too small: the size that is needed
         if (data && total_host > data_bytes) {
+            flags_drop(ctx);  // (the compaction kernel's overflow flag is the same finding)
             raise(VF_ERR_BUFFER_TOO_SMALL, "compressed weights need %llu bytes, buffer holds %llu", (unsigned long long)total_host, (unsigned long long)data_bytes);
         }
         flags_check(ctx);  // synchronises
