@@ -4,7 +4,8 @@ import ctypes as C
 import numpy as np
 import pytest
 
-from test_gpu_blocks import F32, Matrix, device_content, torch, weight_values  # noqa: F401 - torch is a fixture
+import block_reference as br
+from test_gpu_blocks import E4M3, F32, Matrix, device_content, torch, weight_values  # noqa: F401 - torch is a fixture
 from vpux_plugin_b200 import abi
 from vpux_plugin_b200.lib import Library, VfoldError
 
@@ -103,6 +104,20 @@ def test_a_refused_call_keeps_what_a_replay_found(torch):  # noqa: F811
     t.put(t.good)
     t.quantize()
     t.waits_for(abi.VF_ERR_NAN)
+    t.close()
+
+
+def test_a_refused_call_does_not_end_a_recording(torch):  # noqa: F811
+    t = Tokens(torch, 5)
+    t.graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(t.graph, stream=t.stream):
+        refused(t.lib)
+        t.quantize()
+        refused(t.lib)
+    t.replay(t.good)
+    codes, scales = br.quantize(t.good.numpy(), 1, E4M3)
+    assert np.array_equal(t.m.codes()[0], codes) and np.array_equal(t.m.scales()[0], scales)
+    t.waits_for(None)
     t.close()
 
 

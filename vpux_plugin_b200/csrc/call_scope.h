@@ -40,9 +40,15 @@ struct CallScope {  // per-call bookkeeping: context lock, device, error flags, 
         if (stats) stats->kernels_launched = int32_t(ctx->launches - launches0);
     }
     // A call that ends early (an exception on its way to the caller) still waits for what it enqueued: the
-    // caller's buffers and the context's job-table area must not be in use once the call has returned.
+    // caller's buffers and the context's job-table area must not be in use once the call has returned. While the stream is
+    // recorded into a graph nothing of it runs, and a wait would end the recording.
     ~CallScope() {
         if (finished) return;
+        cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+        if (cudaStreamIsCapturing(ctx->main_stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+            cudaGetLastError();
+            return;
+        }
         cudaStreamSynchronize(ctx->main_stream);
         if (ctx->lane_stream) cudaStreamSynchronize(ctx->lane_stream);
         if (ctx->launches != launches0) flags_drop(ctx);
