@@ -1,8 +1,10 @@
 """Refusals of the calls on 8-bit floating-point blocks that need no device, beside those in test_blocks_cpu.py."""
+import numpy as np
 import pytest
 
-from test_blocks_cpu import AT, BF16, matrix, refused
+from test_blocks_cpu import AT, BF16, DEV, E4M3, F32, HOST, matrix, refused
 from vpux_plugin_b200 import abi
+from vpux_plugin_b200.lib import Library
 
 
 @pytest.mark.parametrize("offsets", [8 * AT, 8 * AT + 8, 8 * AT - 24, 8 * AT + 64 - 8])
@@ -36,3 +38,27 @@ def test_more_tiles_than_can_be_counted():
     call(*fine, 1 << 30, 64, 1 << 29)
     call(*fine, 1 << 30, 0)
     call(*fine, 0, 1 << 30)
+
+
+def test_arrays_are_host_memory():
+    """A host address is never handed on as one of device memory."""
+    q, s = np.zeros((4, 256), np.uint8), np.zeros((4, 2), np.float32)
+    assert abi.block_matrix(q, s, E4M3, 1, 4, 256).mem_kind == HOST
+    assert abi.block_matrix(AT, 2 * AT, E4M3, 1, 4, 256).mem_kind == DEV
+    assert abi.block_matrix(None, None, E4M3, 1, 0, 256).mem_kind == DEV
+    assert abi.block_matrix(q, 2 * AT, E4M3, 1, 4, 256, mem_kind=abi.VF_MEM_HOST_PINNED).mem_kind == abi.VF_MEM_HOST_PINNED
+    for args, kw in (((q, s), {"mem_kind": DEV}), ((q, 2 * AT), {}), ((AT, s), {}), ((AT, s), {"mem_kind": DEV}),
+                     ((q, s.astype(np.float64)), {}), ((q.astype(np.int32), s), {}), ((np.zeros((4, 512), np.uint8)[:, ::2], s), {})):
+        with pytest.raises(ValueError):
+            abi.block_matrix(*args, E4M3, 1, 4, 256, **kw)
+
+
+def test_reading_back_into_an_array():
+    """Checked before the library is called: the object below has no context."""
+    lib = Library.__new__(Library)
+    lib.ctx = None
+    m = matrix(4, 256, 1)
+    y = np.zeros((4, 256), np.float32)
+    for dst, nbytes, kw in ((y, y.nbytes, {"dst_mem_kind": DEV}), (y, y.nbytes + 1, {}), (y[:, ::2], 2048, {})):
+        with pytest.raises(ValueError):
+            lib.dequantize_blocks(m, dst, F32, nbytes, **kw)

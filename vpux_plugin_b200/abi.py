@@ -319,13 +319,34 @@ def make_transforms(items):
 VF_BLOCK_COLS = 128
 
 
+def memory_kind(given, *buffers):
+    """The memory kind of buffers that are numpy arrays (host memory) or raw pointers (device memory, unless `given` says
+    otherwise): an address of one kind is never handed on as one of the other."""
+    arrays = pointers = 0
+    for x in buffers:
+        if isinstance(x, np.ndarray):
+            arrays += 1
+            if not x.flags.c_contiguous:
+                raise ValueError("an array has to be C-contiguous")
+        elif x is not None:
+            pointers += 1
+    if not arrays:
+        return VF_MEM_DEVICE if given is None else given
+    if given == VF_MEM_DEVICE:
+        raise ValueError("a numpy array does not live in device memory")
+    if given is None and pointers:
+        raise ValueError("an array beside a raw pointer: mem_kind has to say where they live")
+    return VF_MEM_HOST if given is None else given
+
+
 def block_matrix(codes, scales, dtype, block_rows, rows, cols, count=1, ld=0, matrix_stride=0, scale_row_stride=0,
-                 scale_col_stride=0, scale_matrix_stride=0, mem_kind=VF_MEM_DEVICE, codes_bytes=None, scales_bytes=None):
-    """Build a vf_block_matrix. `codes` and `scales` are raw pointers (device), or numpy arrays (host; keep them alive).
-    Byte sizes that are not given are those of the arrays, or, for raw pointers, exactly what the shape and strides span
+                 scale_col_stride=0, scale_matrix_stride=0, mem_kind=None, codes_bytes=None, scales_bytes=None):
+    """Build a vf_block_matrix. `codes` and `scales` are raw pointers, or numpy arrays (of one-byte elements and of float32;
+    keep them alive). Where `mem_kind` is not given, arrays mean host memory and pointers mean device memory. Byte sizes that are not given are those of the arrays, or, for raw pointers, exactly what the shape and strides span
     (the caller answers for the buffers being that large). With `count` > 1 and scale strides of which the matrix stride
     is missing, the matrices' scales follow one another."""
     m = BlockMatrix()
+    mem_kind = memory_kind(mem_kind, codes, scales)
     row_blocks, col_blocks = -(-rows // block_rows), -(-cols // VF_BLOCK_COLS)
     if (scale_row_stride or scale_col_stride) and not scale_matrix_stride:
         scale_matrix_stride = row_blocks * col_blocks
@@ -334,8 +355,8 @@ def block_matrix(codes, scales, dtype, block_rows, rows, cols, count=1, ld=0, ma
     m.scale_row_stride, m.scale_col_stride, m.scale_matrix_stride = scale_row_stride, scale_col_stride, scale_matrix_stride
     for name, x, given in (("codes", codes, codes_bytes), ("scales", scales, scales_bytes)):
         if isinstance(x, np.ndarray):
-            if not x.flags["C_CONTIGUOUS"]:
-                raise ValueError(f"{name}: the array has to be C-contiguous")
+            if x.dtype.itemsize != 1 if name == "codes" else x.dtype != np.float32:
+                raise ValueError(f"{name}: an array of {x.dtype}")
             setattr(m, name, x.ctypes.data)
             n = x.nbytes
         else:

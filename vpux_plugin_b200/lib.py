@@ -302,8 +302,12 @@ class Library:
         st = self.lib.vf_quantize_blocks(self.ctx, C.byref(content), base_ld, C.byref(out), C.byref(self.last_stats), err, 512)
         self._check(st, err)
 
-    def dequantize_blocks(self, matrix, dst, dst_dtype, dst_bytes, dst_ld=0, dst_mem_kind=abi.VF_MEM_DEVICE):
-        """vf_dequantize_blocks: the values of `matrix` as `dst_dtype` at `dst` (raw pointer, or numpy array in host memory)."""
+    def dequantize_blocks(self, matrix, dst, dst_dtype, dst_bytes, dst_ld=0, dst_mem_kind=None):
+        """vf_dequantize_blocks: the values of `matrix` as `dst_dtype` at `dst` (raw pointer, in device memory unless
+        `dst_mem_kind` says otherwise, or numpy array in host memory)."""
+        dst_mem_kind = abi.memory_kind(dst_mem_kind, dst)
+        if isinstance(dst, np.ndarray) and dst_bytes > dst.nbytes:
+            raise ValueError(f"dst: an array of {dst.nbytes} bytes, not {dst_bytes}")
         err = self._err()
         st = self.lib.vf_dequantize_blocks(self.ctx, C.byref(matrix), _ptr(dst), dst_dtype, dst_ld, dst_bytes, dst_mem_kind,
                                            C.byref(self.last_stats), err, 512)
