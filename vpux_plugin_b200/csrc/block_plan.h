@@ -1,5 +1,5 @@
-// Which rows an expert of a grouped product owns and how many tiles that can make: plain functions that the kernels, the host
-// side and the tests without a device share.
+// Which rows an expert of a grouped product owns, how many tiles that can make, and which form of the product runs: plain functions
+// that the kernels, the host side and the tests share.
 #pragma once
 
 #include <algorithm>
@@ -56,6 +56,58 @@ constexpr int64_t kTileLimit = (int64_t(1) << 31) - (int64_t(1) << 20);
 inline bool too_many_tiles(int64_t rows, int64_t experts, int64_t outputs) {
     const int64_t cols = (outputs + 63) / 64;
     return cols && most_row_tiles(rows, experts, 16) > kTileLimit / cols;
+}
+
+// ---- the forms of the product on the tensor cores -------------------------------------------------------------------------
+// SwapN: the weights are the 128-row operand, N activations the other one, column blocks shared in clusters. WideN: 128 activations by N outputs.
+enum class Form { Swap16, Swap32, Swap128, Wide128, Wide256 };
+
+// The form goes by the rows of activations (of an expert, on average) and by the tiles that there are. Times in us, [rows, outputs, columns]:
+//   up to 16 rows       [16, 4096, 4096]     Swap16 6.5   Swap32 6.9   Swap128 9.4
+//   up to 32            [32, 11008, 4096]    Swap16 13.7  Swap32 11.7  Swap128 19.4; grouped, 32 rows on average, 16 experts [2048, 2048]:
+//                                            Swap32 19.4  Wide128 17.0  Wide256 16.8, since most experts' rows end inside a tile
+//   up to 64, where tiles of 128 x 128 leave half of the multiprocessors idle:
+//                       [64, 4096, 4096]     Swap32 8.3   Swap128 9.6  ([65, 4096, 4096] Wide128 10.8); else
+//                       [64, 11008, 4096]    Swap32 16.4  Swap128 19.9 ([65, 11008, 4096] Wide128 13.1)
+//   above, where they leave three quarters idle:
+//                       [512, 1024, 8192]    Swap128 14.7  Wide128 18.6  Wide256 26.2; else
+//                       [192, 4096, 4096]    Swap128 14.9  Wide128 11.1  Wide256 15.5
+//   and the rest by the rounds that the tiles take; one of Wide256's takes 1.65 times as long as one of Wide128's:
+//                       [512, 4096, 4096]    128 or 64 tiles, one round either way   Wide128 11.8  Wide256 16.7
+//                       [1024, 4096, 4096]   256 or 128 tiles, two rounds or one     Wide128 20.7  Wide256 18.6
+//                       [1500, 4096, 4096]   three rounds or two                     Wide128 29.8  Wide256 31.8
+//                       [4096, 11008, 4096]  nineteen or ten                         Wide128 191.9 Wide256 163.7
+inline Form form_of(int64_t x_rows, int64_t experts, int64_t outputs, int64_t sms) {
+    const int64_t rows = experts ? (x_rows + experts - 1) / experts : x_rows;
+    // (of the experts' last tiles, half are counted: the bound that the grid is sized by counts one for every expert)
+    const int64_t row_tiles = (x_rows + 127) / 128 + experts / 2;
+    const int64_t few = row_tiles * ((outputs + 127) / 128), wide = row_tiles * ((outputs + 255) / 256);
+    if (rows <= 16) return Form::Swap16;
+    if (rows <= 32 && !experts) return Form::Swap32;
+    if (rows <= 64 && few * 2 <= sms) return Form::Swap32;
+    if (few * 4 <= sms) return Form::Swap128;
+    if ((wide + sms - 1) / sms * 165 < (few + sms - 1) / sms * 100) return Form::Wide256;
+    return Form::Wide128;
+}
+
+// Few rows: CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column
+// blocks that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs
+// about as much as four of them. (With tiles of 64 columns, [48, 4096, 11008], 32 tiles of 86 blocks: 40 us alone, 18.7 with four, 13.7
+// with eight, although the last of 32 such clusters has to wait for a place. Clusters of eight CTAs with a multiprocessor each
+// wait more often: [256, 1024, 8192] in 19.6 us with eight, 15.5 with four.)
+//   per_sm    CTAs that a multiprocessor holds
+//   fours     groups of four columns in a tile; the CTAs of a cluster own them in turn, and `places` bounds what all of them keep
+inline int ranks_of(int64_t tiles, int64_t col_blocks, int per_sm, int64_t sms, int fours, int places) {
+    int best = 1;
+    int64_t least = col_blocks;
+    for (int r = 2; r <= 4 * per_sm && 2 * r <= col_blocks && tiles * r <= per_sm * sms; ++r) {
+        const int64_t load = (col_blocks + r - 1) / r + 4;
+        if ((fours + r - 1) / r * r <= places && load < least) {
+            least = load;
+            best = r;
+        }
+    }
+    return best;
 }
 
 }  // namespace vf

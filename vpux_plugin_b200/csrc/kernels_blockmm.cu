@@ -583,61 +583,28 @@ void launch_tensor(vf_ctx* ctx, const BlockProduct& p, int ranks = 1) {
     VF_CUDA(cudaLaunchKernelEx(&cfg, k_matmul_blocks<S, T>, map_codes(p.x, 2, S::kTokens), map_codes(p.w, 3, S::kOutputs), p, int(n_tiles), idesc, ctx->d_flags));
 }
 
-//                    BN, stages, accumulators, epilogue groups of four warps, CTAs per SM, columns per load
+// Forms of block_plan.h: BN, stages, accumulators, epilogue groups of four warps, CTAs per SM, columns per load
 using Swap16 = Shape<true, 16, 5, 4, 1, 2, 16>;
 using Swap32 = Shape<true, 32, 4, 4, 1, 2, 16>;
 using Swap128 = Shape<true, 128, 4, 2, 2, 1, 16>;
 using Wide128 = Shape<false, 128, 5, 2, 2, 1, 32>;
 using Wide256 = Shape<false, 256, 3, 2, 2, 1, 16>;
 
-// Few rows: CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column
-// blocks that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs
-// about as much as four of them. (With tiles of 64 columns, [48, 4096, 11008], 32 tiles of 86 blocks: 40 us alone, 18.7 with four, 13.7
-// with eight, although the last of 32 such clusters has to wait for a place. Clusters of eight CTAs with a multiprocessor each
-// wait more often: [256, 1024, 8192] in 19.6 us with eight, 15.5 with four.)
 template <class S, class T>
 void launch_swapped(vf_ctx* ctx, const BlockProduct& p) {
-    const int64_t tiles = most_tiles(p, S::BN, 128);
-    int best = 1;
-    int64_t least = p.x.col_blocks;
-    for (int r = 2; r <= 4 * S::PER_SM && 2 * r <= p.x.col_blocks && tiles * r <= S::PER_SM * ctx->sm_count; ++r) {
-        const int64_t load = (p.x.col_blocks + r - 1) / r + 4;
-        if ((S::kFours + r - 1) / r * r <= S::kParts && load < least) {
-            least = load;
-            best = r;
-        }
-    }
-    launch_tensor<S, T>(ctx, p, best);
+    launch_tensor<S, T>(ctx, p, ranks_of(most_tiles(p, S::BN, 128), p.x.col_blocks, S::PER_SM, ctx->sm_count, S::kFours, S::kParts));
 }
 
-// The form goes by the rows of activations (of an expert, on average) and by the tiles that there are. Times in us, [rows, outputs, columns]:
-//   up to 16 rows       [16, 4096, 4096]     Swap16 6.5   Swap32 6.9   Swap128 9.4
-//   up to 32            [32, 11008, 4096]    Swap16 13.7  Swap32 11.7  Swap128 19.4; grouped, 32 rows on average, 16 experts [2048, 2048]:
-//                                            Swap32 19.4  Wide128 17.0  Wide256 16.8, since most experts' rows end inside a tile
-//   up to 64, where tiles of 128 x 128 leave half of the multiprocessors idle:
-//                       [64, 4096, 4096]     Swap32 8.3   Swap128 9.6  ([65, 4096, 4096] Wide128 10.8); else
-//                       [64, 11008, 4096]    Swap32 16.4  Swap128 19.9 ([65, 11008, 4096] Wide128 13.1)
-//   above, where they leave three quarters idle:
-//                       [512, 1024, 8192]    Swap128 14.7  Wide128 18.6  Wide256 26.2; else
-//                       [192, 4096, 4096]    Swap128 14.9  Wide128 11.1  Wide256 15.5
-//   and the rest by the rounds that the tiles take; one of Wide256's takes 1.65 times as long as one of Wide128's:
-//                       [512, 4096, 4096]    128 or 64 tiles, one round either way   Wide128 11.8  Wide256 16.7
-//                       [1024, 4096, 4096]   256 or 128 tiles, two rounds or one     Wide128 20.7  Wide256 18.6
-//                       [1500, 4096, 4096]   three rounds or two                     Wide128 29.8  Wide256 31.8
-//                       [4096, 11008, 4096]  nineteen or ten                         Wide128 191.9 Wide256 163.7
 template <class T>
 void launch_for(vf_ctx* ctx, const BlockProduct& p) {
     if (!fits_bulk_copies(p.x) || !fits_bulk_copies(p.w)) return launch_plain<T>(ctx, p);
-    const int64_t rows = p.offsets ? (p.x.rows + p.w.count - 1) / p.w.count : p.x.rows, sms = ctx->sm_count;
-    // (of the experts' last tiles, half are counted: the bound that the grid is sized by counts one for every expert)
-    const int64_t row_tiles = (p.x.rows + 127) / 128 + (p.offsets ? p.w.count / 2 : 0);
-    const int64_t few = row_tiles * ((p.w.rows + 127) / 128), wide = row_tiles * ((p.w.rows + 255) / 256);
-    if (rows <= 16) return launch_swapped<Swap16, T>(ctx, p);
-    if (rows <= 32 && !p.offsets) return launch_swapped<Swap32, T>(ctx, p);
-    if (rows <= 64 && few * 2 <= sms) return launch_swapped<Swap32, T>(ctx, p);
-    if (few * 4 <= sms) return launch_swapped<Swap128, T>(ctx, p);
-    if ((wide + sms - 1) / sms * 165 < (few + sms - 1) / sms * 100) return launch_tensor<Wide256, T>(ctx, p);
-    launch_tensor<Wide128, T>(ctx, p);
+    switch (form_of(p.x.rows, p.offsets ? p.w.count : 0, p.w.rows, ctx->sm_count)) {
+    case Form::Swap16: return launch_swapped<Swap16, T>(ctx, p);
+    case Form::Swap32: return launch_swapped<Swap32, T>(ctx, p);
+    case Form::Swap128: return launch_swapped<Swap128, T>(ctx, p);
+    case Form::Wide128: return launch_tensor<Wide128, T>(ctx, p);
+    case Form::Wide256: return launch_tensor<Wide256, T>(ctx, p);
+    }
 }
 
 }  // namespace
