@@ -388,7 +388,8 @@ int vf_quantize_fold(vf_ctx* ctx, const vf_content* base, const vf_quant_spec* s
  * block_rows is 128 for weights (one scale per 128 x 128 block) and 1 for activations (one per 128 columns of a
  * row). The last block of a row or column may be short. ld = 0 stands for `cols`, matrix_stride = 0 for rows * ld,
  * and three scale strides of 0 for a dense array [count][row blocks][column blocks]. Strides count elements, are
- * not negative and let no two elements meet. The reference's quantized types hold one scale per index of one axis
+ * not negative and nested (each steps over all that the smaller ones reach), so that no two elements meet; the buffers of a
+ * call do not overlap, from the first to the last element of each. The reference's quantized types hold one scale per index of one axis
  * (!quant.uniform<storage:expressed:axis>); this is the form for which the library's own products exist. */
 #define VF_BLOCK_COLS 128
 typedef struct vf_block_matrix {
@@ -410,7 +411,7 @@ typedef struct vf_block_matrix {
  * element (i * rows + r) * base_ld; base_ld = 0 stands for cols) into `out`, whose shape must agree:
  *     scale = max(fl(absmax of the block / L), 2^-126)      L = 448 (e4m3), 57344 (e5m2)
  *     code  = nearest 8-bit float, ties to even, of fl(x * fl(1 / scale))
- * so the largest magnitude of a block becomes +-L and a block of zeros gets the scale 2^-126. Bytes of `out` between
+ * so the largest magnitude of a block becomes +-L (unless the scale is held at 2^-126) and a block of zeros gets the scale 2^-126. Bytes of `out` between
  * rows are left as they are. A NaN gives VF_ERR_NAN, an infinity VF_ERR_QUANT_RANGE, both after the kernel ran (the
  * block's outputs are then unspecified, the others are complete). */
 int vf_quantize_blocks(vf_ctx* ctx, const vf_content* base, int64_t base_ld, const vf_block_matrix* out, vf_stats* stats,
@@ -425,7 +426,7 @@ int vf_dequantize_blocks(vf_ctx* ctx, const vf_block_matrix* in, void* dst, int3
 /* y[m][n] = sum over k of x[m][k] * w[n][k]: activations x [M, K] with block_rows 1, weights w [N, K] with block_rows
  * 128 (either 8-bit type on either side), y as `out_dtype` (VF_DT_F32 / F16 / BF16) with rows `out_ld` elements apart
  * (0 = N). Per 128 columns the codes are multiplied and summed in fp32, the sum is scaled by the product of the two scales
- * and added in fp32; y is rounded once, to nearest even, overflow to infinity. Everything lives in DEVICE memory;
+ * (an fp32 number as well: scales whose product leaves the range of normal ones lose it) and added in fp32; y is rounded once, to nearest even, overflow to infinity. Everything lives in DEVICE memory;
  * M = 0 or N = 0 writes nothing. Operands whose codes start on 16-byte boundaries with `ld` (and matrix_stride) a
  * multiple of 16 run on the tensor cores, others on a plain kernel that is tens of times slower. Tiles are counted in 32
  * bits: a claim of more than 2^31 - 2^20 tiles of 16 rows by 64 columns, more than the device's memory holds, is refused

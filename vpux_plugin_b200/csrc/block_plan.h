@@ -62,7 +62,8 @@ inline bool too_many_tiles(int64_t rows, int64_t experts, int64_t outputs) {
 // SwapN: the weights are the 128-row operand, N activations the other one, column blocks shared in clusters. WideN: 128 activations by N outputs.
 enum class Form { Swap16, Swap32, Swap128, Wide128, Wide256 };
 
-// The form goes by the rows of activations (of an expert, on average) and by the tiles that there are. Times in us, [rows, outputs, columns]:
+// The form goes by the rows of activations (of an expert, on average) and by the tiles that there are. Times in us of short bursts
+// replayed from a graph (the power limit slows both sides of a long run alike), [rows, outputs, columns]:
 //   up to 16 rows       [16, 4096, 4096]     Swap16 6.5   Swap32 6.9   Swap128 9.4
 //   up to 32            [32, 11008, 4096]    Swap16 13.7  Swap32 11.7  Swap128 19.4; grouped, 32 rows on average, 16 experts [2048, 2048]:
 //                                            Swap32 19.4  Wide128 17.0  Wide256 16.8, since most experts' rows end inside a tile
@@ -92,9 +93,13 @@ inline Form form_of(int64_t x_rows, int64_t experts, int64_t outputs, int64_t sm
 
 // Few rows: CTAs that share a tile's column blocks, where every tile can have a cluster of its own. A CTA's time goes with the column
 // blocks that it walks through one after the other, whether another CTA shares its multiprocessor or not; joining costs
-// about as much as four of them. (With tiles of 64 columns, [48, 4096, 11008], 32 tiles of 86 blocks: 40 us alone, 18.7 with four, 13.7
-// with eight, although the last of 32 such clusters has to wait for a place. Clusters of eight CTAs with a multiprocessor each
-// wait more often: [256, 1024, 8192] in 19.6 us with eight, 15.5 with four.)
+// about as much as four of them. In us by CTAs per cluster, the rule's choice marked (the same bursts; "more" than there is room for):
+//   Swap16   [1, 4096, 4096]      1: 10.1  2: 7.3   3: 6.4   4: 6.1   6: 6.0   8: 6.3 *
+//            [1, 11008, 4096]     1: 12.6  2: 11.9  3: 10.1 *  4: 14.4 more  8: 18.1 more
+//            [16, 4096, 11008]    1: 22.7  2: 15.2  4: 11.7  6: 11.3  8: 10.9 *
+//   Swap32   [48, 4096, 11008]    1: 31.5  2: 20.1  3: 15.8  4: 14.0 *  5: 21.1 more  8: 19.7 more
+//            [64, 1024, 8192]     1: 20.3  2: 12.9  4: 9.3   8: 7.5 *
+//   Swap128  [256, 1024, 8192]    1: 32.3  2: 20.9  4: 13.7 *  8: 20.1 (clusters of eight CTAs with a multiprocessor each wait more often)
 //   per_sm    CTAs that a multiprocessor holds
 //   fours     groups of four columns in a tile; the CTAs of a cluster own them in turn, and `places` bounds what all of them keep
 inline int ranks_of(int64_t tiles, int64_t col_blocks, int per_sm, int64_t sms, int fours, int places) {

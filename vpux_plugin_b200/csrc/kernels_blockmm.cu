@@ -95,11 +95,12 @@ void launch_plain(vf_ctx* ctx, const BlockProduct& p) {
 // tiles and copies them in (bulk tensor copies into a ring of STAGES), one that issues the matrix instructions, and one that
 // brings the scales of eight column blocks at a time into a ring of their own.
 //
-// Measured ([rows, outputs, columns], back to back, graph replay): [4096, 11008, 4096] 161-164 us, 2.3 PFLOP/s, tensor pipe active 64 % of the time; about 820 cycles per
-// column block and tile, of which the tensor core needs 512. What bounds it: two accumulators of 256 columns fill the tensor
-// memory, and from one use of an accumulator to the next pass the instructions (512), the epilogue's 480 cycles of reading it
-// and three hand-overs through barriers; and the power limit (the clock falls to 1.6 GHz under this load).
-// Tried before the issuing warp became uniform, when this size took 180: pairs of CTAs (256 x 256 tiles) 177-184 us, 128 x 192 tiles
+// Measured ([rows, outputs, columns]): [4096, 11008, 4096] 192 us in calls that follow one another for seconds, 1.93 PFLOP/s, at the
+// 1.43 GHz that the power limit then leaves; 166 us in bursts of 84 launches from idle. That is about 860 cycles per column block and
+// tile, of which the tensor core needs 512 (tensor pipe active 64 % of the time). What bounds it: two accumulators of 256 columns fill the
+// tensor memory, and from one use of an accumulator to the next pass the instructions (512), the epilogue's 480 cycles of reading it
+// and three hand-overs through barriers; and the power limit.
+// Tried before the issuing warp became uniform, when this size took 180 in bursts, and not since: pairs of CTAs (256 x 256 tiles) 177-184 us, 128 x 192 tiles
 // 206, four epilogue groups 193-199, 32 columns per load 190, the column-block loop unrolled twice 221-290 (it spills).
 // [1, 11008, 4096] 10.1 us and [48, 4096, 11008] 13.9 us at 4.5 and 3.3 TB/s of weights; [1, 32000, 8192] 43.4 us at 6.0 TB/s: a
 // launch costs 3.5 us of its own, and joining the CTAs of a cluster 1 to 3.
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(S::kThreads, S::PER_SM)
 
     // What is the same for a whole warp comes from one lane: the compiler then knows that it is, keeps the warps' branches and the
     // operands of the matrix and copy instructions uniform, and a column block's four instructions and two commits are issued in
-    // half the time ([4096, 11008, 4096] 180 -> 165 us, [400, 4096, 11008] 37 -> 26 us).
+    // half the time ([4096, 11008, 4096] 180 -> 165 us in bursts, [400, 4096, 11008] 37 -> 26 us).
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x) >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t ranks = S::SWAP ? __shfl_sync(0xffffffffu, cluster_size(), 0) : 1, rank = S::SWAP ? __shfl_sync(0xffffffffu, cluster_rank(), 0) : 0;  // CTAs that share a tile's column blocks
     const bool in_cluster = ranks > 1;
