@@ -14,6 +14,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
+// (The kernels' inputs are not declared __restrict__: the compiler would read them through the path for data that nobody writes while
+// the kernel runs, but these kernels start while the one that writes their input still does.)
 template <class T>
 struct Eight {  // eight consecutive elements of a row, as 32-bit words
     static constexpr int kWords = sizeof(T) * 2;
@@ -127,7 +129,7 @@ __device__ __forceinline__ void store_codes(uint8_t* p, uint2 c, int n) {
 //   [8192, 11008] bf16: 43.9 us with eight rows (6.2 TB/s), 54.9 with four, 60.6 with two; 59 us with four when every lane divided
 //   for every row. [1, 4096]: 2.5 us with eight, 1.6 with two. Bound by memory (issue slots 62 % busy).
 template <class T, int Rows, bool E5M2, bool Aligned>
-__global__ void __launch_bounds__(kThreads, 4) k_quantize_tokens(const T* __restrict__ base, int64_t base_ld, Blocks b, int64_t col_tiles, int64_t tiles,
+__global__ void __launch_bounds__(kThreads, 4) k_quantize_tokens(const T* base, int64_t base_ld, Blocks b, int64_t col_tiles, int64_t tiles,
                                                                  int* flags) {
     chain_enter();
     constexpr int kShare = 16 / Rows;  // lanes that end up with the same row
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_quantize_tokens(const T* __rest
 // 118 us, 6.0 TB/s: 2752 tiles make 4.6 rounds). Tried: 512 threads with four loads each 27.7, five CTAs per multiprocessor 28.7 (it
 // spills), a persistent grid 26.9, rows of blocks before columns 28.0.
 template <class T, bool E5M2, bool Aligned>
-__global__ void __launch_bounds__(kThreads) k_quantize_weights(const T* __restrict__ base, int64_t base_ld, Blocks b, int64_t tiles, int* flags) {
+__global__ void __launch_bounds__(kThreads) k_quantize_weights(const T* base, int64_t base_ld, Blocks b, int64_t tiles, int* flags) {
     chain_enter();
     constexpr int kIter = kBlock / (kThreads / 16);
     __shared__ uint32_t tops[2][kThreads / 32];
